@@ -64,12 +64,47 @@ class FmInfo(C.Structure):
     ]
 
 
+# element types of the operators' buffers (include/factorysim.h FM_DTYPE_*)
+FM_DTYPE_F32, FM_DTYPE_F16, FM_DTYPE_BF16, FM_DTYPE_F64, FM_DTYPE_I32, FM_DTYPE_I64 = range(6)
+FM_DISTILL_MAX_K = 1024
+
+_I, _Q, _D, _P = C.c_int32, C.c_int64, C.c_double, C.c_void_p
+
+
+class FmLayerNormArgs(C.Structure):
+    _fields_ = [("device", _I), ("x_dtype", _I), ("param_dtype", _I), ("reserved", _I), ("rows", _Q), ("cols", _Q),
+                ("x", _P), ("x_stride", _Q), ("weight", _P), ("bias", _P), ("eps", _D), ("y", _P), ("mean", _P),
+                ("rstd", _P), ("dy", _P), ("dy_stride", _Q), ("dx", _P), ("dweight", _P), ("dbias", _P),
+                ("workspace", _P), ("workspace_bytes", _Q), ("stream", _P)]
+
+
+class FmSampleArgs(C.Structure):
+    _fields_ = [("device", _I), ("dtype", _I), ("u_dtype", _I), ("reserved", _I), ("rows", _Q), ("cols", _Q),
+                ("logits", _P), ("stride", _Q), ("mask", _P), ("mask_stride", _Q), ("u", _P), ("temperature", _D),
+                ("top_p", _D), ("min_p", _D), ("top_k", _Q), ("temperature_rows", _P), ("top_p_rows", _P),
+                ("min_p_rows", _P), ("top_k_rows", _P), ("out", _P), ("workspace", _P), ("workspace_bytes", _Q),
+                ("stream", _P)]
+
+
+class FmDistillArgs(C.Structure):
+    _fields_ = [("device", _I), ("dtype", _I), ("index_dtype", _I), ("teacher_dtype", _I), ("rows", _Q), ("cols", _Q),
+                ("k", _Q), ("logits", _P), ("stride", _Q), ("index", _P), ("index_stride", _Q), ("teacher", _P),
+                ("teacher_stride", _Q), ("temperature", _D), ("loss", _P), ("stats", _P), ("grad", _P),
+                ("grad_stride", _Q), ("dlogits", _P), ("workspace", _P), ("workspace_bytes", _Q), ("stream", _P)]
+
+
+OPERATORS = {  # entry point -> its argument record; the workspace sizes below
+    "fm_layer_norm_forward": FmLayerNormArgs, "fm_layer_norm_backward": FmLayerNormArgs,
+    "fm_sample_logits": FmSampleArgs, "fm_distill_forward": FmDistillArgs, "fm_distill_backward": FmDistillArgs,
+}
+WORKSPACES = ("fm_layer_norm_workspace", "fm_sample_workspace", "fm_distill_workspace")
+
 EXPORTED = [
     "fm_config_default", "fm_create", "fm_destroy", "fm_last_error", "fm_set_stream", "fm_sync", "fm_obs_dim",
     "fm_act_dim", "fm_num_arenas", "fm_nq", "fm_nv", "fm_nu", "fm_workspace_bytes", "fm_reset", "fm_step", "fm_state_size",
     "fm_get_state", "fm_set_state", "fm_get_counters", "fm_debug_dump", "fm_profile", "fm_scene_mjcf",
     "fm_render", "fm_render_ngeom", "fm_set_param", "fm_get_param", "fm_num_counters", "fm_get_costs",
-    "fm_kernel_timing", "fm_get_kernel_time", "fm_abi_version", "fm_config_size",
+    "fm_kernel_timing", "fm_get_kernel_time", "fm_abi_version", "fm_config_size", *OPERATORS, *WORKSPACES,
 ]
 ABI_VERSION = 2  # include/factorysim.h FM_ABI_VERSION
 
@@ -146,6 +181,13 @@ def load(experimental=False):
     if hasattr(L, "fm_num_counters"):
         L.fm_num_counters.argtypes = []
         L.fm_num_counters.restype = I
+    if hasattr(L, "fm_layer_norm_forward"):  # libraries before the operators still step environments
+        for n, args in OPERATORS.items():
+            getattr(L, n).argtypes = [C.POINTER(args)]
+            getattr(L, n).restype = I
+        for n in WORKSPACES:
+            getattr(L, n).argtypes = [_Q, _Q]
+            getattr(L, n).restype = _Q
     _LIBS[path] = L
     return L
 

@@ -70,6 +70,17 @@ static int set_err(int code, const std::string& msg) {
   return code;
 }
 
+// the operators' objects (fm_norm.hip, fm_sample.hip, fm_distill.hip) report through the same text
+namespace fm {
+int report(int code, const char* msg) noexcept {
+  try {
+    return set_err(code, msg);
+  } catch (...) {
+    return code;
+  }
+}
+}  // namespace fm
+
 #define HIPCHK(x)                                                                                  \
   do {                                                                                             \
     hipError_t e_ = (x);                                                                           \

@@ -1,0 +1,304 @@
+"""Operators of a policy's head on the library's own kernels (include/factorysim.h, fm_norm.hip / fm_sample.hip /
+fm_distill.hip): layer norm, drawing categories from logits, distillation from a teacher's top logits.
+
+GPU tensors are computed on torch's current stream of their device, CPU tensors by the library's CPU backend (as
+``FactoryVecEnv(device=-1)``); there is no other path, a missing library raises.  Inputs may have any leading shape and
+row stride; one whose last dimension is not adjacent in memory is copied first.  Nothing synchronises and no buffer is kept between
+calls, so each call, forward or backward, can be captured into a graph.  A backward pass that is captured needs leaves
+that no live eager graph holds: torch ties a leaf's gradient to the stream of the graph that first used it.
+"""
+import math
+
+import torch
+import torch.nn as nn
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+
+__all__ = ["layer_norm", "LayerNorm", "sample_logits", "distill_loss", "MAX_LISTED"]
+
+MAX_LISTED = _lib.FM_DISTILL_MAX_K  # most categories that distill_loss takes for a row
+
+_DTYPES = {torch.float32: _lib.FM_DTYPE_F32, torch.float16: _lib.FM_DTYPE_F16, torch.bfloat16: _lib.FM_DTYPE_BF16}
+_INDEX = {torch.int32: _lib.FM_DTYPE_I32, torch.int64: _lib.FM_DTYPE_I64}
+
+
+def _library():
+    L = _lib.load()
+    if not hasattr(L, "fm_layer_norm_forward"):
+        raise _lib.FactorySimError(f"{_lib.LIB_PATH} has no operators: rebuild it")
+    return L
+
+
+def _where(t):
+    """(device ordinal or -1, stream) of a tensor's calls"""
+    if t.is_cuda:
+        d = t.device.index
+        return d, torch._C._cuda_getCurrentRawStream(d)
+    if t.device.type != "cpu":
+        raise ValueError(f"tensors are on a GPU or the CPU, not on {t.device}")
+    return -1, None
+
+
+def _rows(t):
+    """t as [rows, cols] with adjacent columns: a view where there is one"""
+    if t.dim() != 2:
+        n = t.shape[-1]
+        t = t.reshape(-1 if n else 0, n)
+    return t if t.shape[1] <= 1 or t.stride(1) == 1 else t.contiguous()
+
+
+def _stride(t):
+    return t.stride(0) if t.shape[0] > 1 else 0
+
+
+def _float_input(name, t):
+    if not torch.is_tensor(t):
+        raise TypeError(f"{name} is a tensor")
+    if t.dtype not in _DTYPES:
+        raise TypeError(f"{name} is float32, float16 or bfloat16, not {t.dtype}")
+    if t.dim() < 1 or t.shape[-1] < 1:
+        raise ValueError(f"{name} needs a last dimension of at least 1, got shape {tuple(t.shape)}")
+
+
+def _same_device(t, **others):
+    for name, o in others.items():
+        if o is not None and o.device != t.device:
+            raise ValueError(f"{name} is on {o.device}, the first input on {t.device}")
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+# ------------------------------------------------------------------ layer norm
+def _norm_forward(x, weight, bias, eps, keep):
+    L = _library()
+    dev, stream = _where(x)
+    n, v = x.shape
+    y = torch.empty((n, v), dtype=x.dtype, device=x.device)
+    stats = torch.empty((2, n), dtype=torch.float32, device=x.device) if keep else None
+    mean = _ptr(stats)
+    p = weight if weight is not None else bias
+    a = _lib.FmLayerNormArgs(dev, _DTYPES[x.dtype], _DTYPES[x.dtype if p is None else p.dtype], 0, n, v, x.data_ptr(),
+                             _stride(x), _ptr(weight), _ptr(bias), eps, y.data_ptr(), mean,
+                             mean + 4 * n if keep else None, None, 0, None, None, None, None, 0, stream)
+    _lib.check(L.fm_layer_norm_forward(a), L)
+    return y, stats
+
+
+class _LayerNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps):
+        y, stats = _norm_forward(x, weight, bias, eps, True)
+        ctx.save_for_backward(x, weight, stats)
+        ctx.bias_dtype = None if bias is None else bias.dtype
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, weight, stats = ctx.saved_tensors
+        L = _library()
+        dev, stream = _where(x)
+        n, v = x.shape
+        dy = _rows(dy)
+        want_x, want_w, want_b = ctx.needs_input_grad[:3]
+        pt = weight.dtype if weight is not None else ctx.bias_dtype or x.dtype
+        dx = torch.empty((n, v), dtype=x.dtype, device=x.device) if want_x else None
+        dw = torch.empty(v, dtype=pt, device=x.device) if want_w else None
+        db = torch.empty(v, dtype=pt, device=x.device) if want_b else None
+        need = L.fm_layer_norm_workspace(n, v) if (want_w or want_b) and dev >= 0 else 0
+        work = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
+        mean = stats.data_ptr()
+        a = _lib.FmLayerNormArgs(dev, _DTYPES[x.dtype], _DTYPES[pt], 0, n, v, x.data_ptr(), _stride(x), _ptr(weight),
+                                 None, 0.0, None, mean, mean + 4 * n, dy.data_ptr(), _stride(dy), _ptr(dx), _ptr(dw),
+                                 _ptr(db), _ptr(work), need, stream)
+        _lib.check(L.fm_layer_norm_backward(a), L)
+        return dx, dw, db, None
+
+
+def layer_norm(x, weight=None, bias=None, eps=1e-5):
+    """(x - mean) / sqrt(variance + eps) * weight + bias over the last dimension (biased variance), in x's dtype.
+
+    x: float32, float16 or bfloat16; weight, bias: [x.shape[-1]], both of x's dtype or both float32, or None.  Statistics
+    and sums are held in 32 bits and each result is rounded once.  Differentiable once in x, weight and bias; the
+    parameters' gradients are summed over rows in a fixed order."""
+    _float_input("x", x)
+    v = x.shape[-1]
+    for name, p in (("weight", weight), ("bias", bias)):
+        if p is None:
+            continue
+        if p.dtype != x.dtype and p.dtype != torch.float32:
+            raise TypeError(f"{name} is float32 or of x's dtype {x.dtype}, not {p.dtype}")
+        if tuple(p.shape) != (v,):
+            raise ValueError(f"{name} has shape {tuple(p.shape)}, x's last dimension is {v}")
+    if weight is not None and bias is not None and weight.dtype != bias.dtype:
+        raise TypeError(f"weight is {weight.dtype}, bias {bias.dtype}: one dtype for both")
+    _same_device(x, weight=weight, bias=bias)
+    eps = float(eps)
+    if not 0 <= eps < math.inf:
+        raise ValueError(f"eps is finite and not negative, got {eps}")
+    w = weight if weight is None or weight.is_contiguous() else weight.contiguous()
+    b = bias if bias is None or bias.is_contiguous() else bias.contiguous()
+    x2 = _rows(x)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x2, w, b)):
+        y = _LayerNorm.apply(x2, w, b, eps)
+    else:
+        y = _norm_forward(x2, w, b, eps, False)[0]
+    return y if x.dim() == 2 else y.view(x.shape)
+
+
+class LayerNorm(nn.Module):
+    """``layer_norm`` over the last dimension with a weight (ones at first) and a bias (zeros)"""
+
+    def __init__(self, dim, eps=1e-5):
+        super().__init__()
+        self.eps = eps
+        self.weight = nn.Parameter(torch.ones(dim))
+        self.bias = nn.Parameter(torch.zeros(dim))
+
+    def forward(self, x):
+        return layer_norm(x, self.weight, self.bias, self.eps)
+
+    def extra_repr(self):
+        return f"{self.weight.numel()}, eps={self.eps}"
+
+
+# ------------------------------------------------------------------ drawing categories
+def _setting(name, value, rows, logits, dtype):
+    """(number, None) or (0, tensor of one number a row)"""
+    if not torch.is_tensor(value):
+        return (int(value) if dtype == torch.int32 else float(value)), None
+    if value.dtype.is_floating_point != (dtype == torch.float32) or value.dtype in (torch.bool, torch.float64):
+        raise TypeError(f"{name} of each row is {'a float32' if dtype == torch.float32 else 'an integer'} tensor, not {value.dtype}")
+    if value.numel() != rows or (value.dim() > 1 and value.shape != logits.shape[:-1]):
+        raise ValueError(f"{name} has shape {tuple(value.shape)}, the logits' rows {tuple(logits.shape[:-1])}")
+    if value.dtype == torch.int64:  # beyond any number of categories is off, as 0 is
+        value = value.clamp(0, 2**31 - 1)
+    return 0, value.reshape(-1).to(dtype).contiguous()
+
+
+@torch.no_grad()
+def sample_logits(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, mask=None):
+    """One category of each row of ``logits`` [..., categories], drawn with the uniform numbers ``u`` [...]: int64 [...].
+
+    A row's categories are ranked by logit, the lower index first among equals, and weigh exp(logit / temperature).
+    ``top_k`` keeps the first k, ``top_p`` the shortest leading part of those that holds at least that share of their
+    weight, ``min_p`` those of them that weigh at least that share of the largest.  The result is the first of the kept
+    categories, in rank, up to which more than the share u of their weight lies: u = 0 gives the largest logit.
+
+    Each setting is a number or a tensor with one number for each row (float32; ``top_k`` integer).  temperature <= 0
+    gives the largest logit; top_k <= 0, top_p >= 1 and min_p <= 0 are off.  ``mask`` (bool, logits' shape or
+    [categories]) bars categories where it is False, whatever their logit; a logit of -inf bars its category too.
+    -1 stands for a row with no category left, with NaN in a logit that is not barred, or with a NaN in u or a setting.  logits: float32,
+    float16 or bfloat16; u: float32 or float64, in [0, 1).  Weights below 2^-46 of the largest count as nothing."""
+    _float_input("logits", logits)
+    if not torch.is_tensor(u) or u.dtype not in (torch.float32, torch.float64):
+        raise TypeError("u is a float32 or float64 tensor")
+    if u.shape != logits.shape[:-1]:
+        raise ValueError(f"u has shape {tuple(u.shape)}, the logits' rows {tuple(logits.shape[:-1])}")
+    _same_device(logits, u=u, mask=mask, **{n: s for n, s in (("temperature", temperature), ("top_k", top_k),
+                                                               ("top_p", top_p), ("min_p", min_p)) if torch.is_tensor(s)})
+    z = _rows(logits)
+    n, v = z.shape
+    m = None
+    if mask is not None:
+        if mask.dtype != torch.bool:
+            raise TypeError(f"mask is a bool tensor, not {mask.dtype}")
+        if mask.shape != logits.shape and tuple(mask.shape) != (v,):
+            raise ValueError(f"mask has shape {tuple(mask.shape)}, the logits {tuple(logits.shape)}")
+        m = _rows(mask if mask.shape == logits.shape else mask[None])
+    t, t_rows = _setting("temperature", temperature, n, logits, torch.float32)
+    k, k_rows = _setting("top_k", top_k, n, logits, torch.int32)
+    p, p_rows = _setting("top_p", top_p, n, logits, torch.float32)
+    q, q_rows = _setting("min_p", min_p, n, logits, torch.float32)
+    if t != t or p != p or q != q:
+        raise ValueError("temperature, top_p and min_p are numbers, not NaN")
+    u = u.reshape(-1).contiguous()
+    L = _library()
+    dev, stream = _where(logits)
+    out = torch.empty(logits.shape[:-1], dtype=torch.int64, device=logits.device)
+    need = L.fm_sample_workspace(n, v) if dev >= 0 else 0
+    work = torch.empty(need, dtype=torch.uint8, device=logits.device) if need else None
+    a = _lib.FmSampleArgs(dev, _DTYPES[z.dtype], _lib.FM_DTYPE_F32 if u.dtype == torch.float32 else _lib.FM_DTYPE_F64, 0,
+                          n, v, z.data_ptr(), _stride(z), _ptr(m), 0 if m is None else _stride(m), u.data_ptr(), t, p,
+                          q, min(max(k, 0), 2**31 - 1), _ptr(t_rows), _ptr(p_rows), _ptr(q_rows), _ptr(k_rows), out.data_ptr(),
+                          _ptr(work), need, stream)
+    _lib.check(L.fm_sample_logits(a), L)
+    return out
+
+
+# ------------------------------------------------------------------ distillation
+def _distill_args(z, index, teacher, temperature):
+    dev, stream = _where(z)
+    n, v = z.shape
+    return _lib.FmDistillArgs(dev, _DTYPES[z.dtype], _INDEX[index.dtype], _DTYPES[teacher.dtype], n, v, index.shape[1],
+                              z.data_ptr(), _stride(z), index.data_ptr(), _stride(index), teacher.data_ptr(),
+                              _stride(teacher), temperature, None, None, None, 0, None, None, 0, stream)
+
+
+def _distill_forward(z, index, teacher, temperature, keep):
+    L = _library()
+    a = _distill_args(z, index, teacher, temperature)
+    n = z.shape[0]
+    loss = torch.empty(n, dtype=torch.float32, device=z.device)
+    stats = torch.empty((n, 2), dtype=torch.float32, device=z.device) if keep else None
+    need = L.fm_distill_workspace(n, z.shape[1]) if a.device >= 0 else 0
+    work = torch.empty(need, dtype=torch.uint8, device=z.device) if need else None
+    a.loss, a.stats, a.workspace, a.workspace_bytes = loss.data_ptr(), _ptr(stats), _ptr(work), need
+    _lib.check(L.fm_distill_forward(a), L)
+    return loss, stats
+
+
+class _Distill(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, z, index, teacher, temperature):
+        loss, stats = _distill_forward(z, index, teacher, temperature, True)
+        ctx.save_for_backward(z, index, teacher, stats)
+        ctx.temperature = temperature
+        return loss
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        z, index, teacher, stats = ctx.saved_tensors
+        L = _library()
+        a = _distill_args(z, index, teacher, ctx.temperature)
+        dz = torch.empty(z.shape, dtype=z.dtype, device=z.device)
+        a.stats, a.grad, a.grad_stride, a.dlogits = stats.data_ptr(), grad.data_ptr(), grad.stride(0), dz.data_ptr()
+        _lib.check(L.fm_distill_backward(a), L)
+        return dz, None, None, None
+
+
+def distill_loss(logits, teacher_index, teacher_logits, temperature=1.0):
+    """temperature^2 times the Kullback-Leibler divergence of softmax(logits / temperature) over all categories from
+    softmax(teacher_logits / temperature) over the listed ones, for each row: float32 [...].
+
+    logits [..., categories] (float32, float16 or bfloat16); teacher_index [..., k] (int32 or int64) names the listed
+    categories and teacher_logits [..., k] (a float dtype of its own) their logits, k at most 1024, in any order.  An
+    entry with a negative index or a teacher logit of -inf is not listed (lists of unequal length are padded so); a row
+    with none has loss 0 and gradient 0.  A category listed twice counts twice.  An index that is no category cannot be raised
+    without waiting for the GPU: it makes its row's loss and gradient NaN.  Differentiable once in the logits; the
+    teacher's logits are constants."""
+    _float_input("logits", logits)
+    _float_input("teacher_logits", teacher_logits)
+    if not torch.is_tensor(teacher_index) or teacher_index.dtype not in _INDEX:
+        raise TypeError("teacher_index is an int32 or int64 tensor")
+    if teacher_index.shape != teacher_logits.shape or teacher_index.shape[:-1] != logits.shape[:-1]:
+        raise ValueError(f"teacher_index {tuple(teacher_index.shape)} and teacher_logits {tuple(teacher_logits.shape)} "
+                         f"list categories for each row of the logits {tuple(logits.shape)}")
+    if teacher_index.shape[-1] > MAX_LISTED:
+        raise ValueError(f"at most {MAX_LISTED} categories can be listed, got {teacher_index.shape[-1]}")
+    if teacher_logits.requires_grad:
+        raise ValueError("teacher_logits requires a gradient, which this loss does not give: detach it")
+    _same_device(logits, teacher_index=teacher_index, teacher_logits=teacher_logits)
+    temperature = float(temperature)
+    if not 1e-30 <= temperature <= 1e30:
+        raise ValueError(f"temperature is positive and within 1e-30 .. 1e30, got {temperature}")
+    z, index, teacher = _rows(logits), _rows(teacher_index), _rows(teacher_logits)
+    if torch.is_grad_enabled() and z.requires_grad:
+        loss = _Distill.apply(z, index, teacher, temperature)
+    else:
+        loss = _distill_forward(z, index, teacher, temperature, False)[0]
+    return loss if logits.dim() == 2 else loss.view(logits.shape[:-1])

@@ -20,6 +20,11 @@ this image, so this module restates the parts of SB3 2.3.2 the reference uses, o
   for [128, 128]).  Episode statistics are all-reduced once per rollout.  With the "nccl" backend the
   collectives are RCCL over xGMI.
 
+Beyond SB3, off unless asked for, on the library's operators (ops.py): ``layer_norm`` normalises every hidden layer
+before its tanh; ``fused_sampling`` draws all of a MultiDiscrete policy's actions in one launch; ``predict`` takes
+temperature / top_k / top_p / min_p; ``PPO(teacher=...)`` adds a distillation term towards another MultiDiscrete
+policy (a saved run's, say), whose top logits are recorded in the rollout.
+
 n_steps / batch_size: SB3's 2048 x 64 does not scale to 16k-131k arenas; the caller chooses them (defaults here:
 n_steps 16, batch_size 8192 per rank) and they are recorded in ``data`` of every checkpoint.
 """
@@ -33,17 +38,19 @@ import numpy as np
 import torch
 import torch.nn as nn
 
+from . import ops
+
 __all__ = ["ActorCriticPolicy", "PPO", "load_sb3_policy_state", "flat_allreduce", "compute_gae"]
 
 
 class _MlpExtractor(nn.Module):
-    def __init__(self, obs_dim, net_arch):
+    def __init__(self, obs_dim, net_arch, layer_norm=False):
         super().__init__()
 
         def mlp():
             layers, last = [], obs_dim
             for h in net_arch:
-                layers += [nn.Linear(last, h), nn.Tanh()]
+                layers += [nn.Linear(last, h), ops.LayerNorm(h), nn.Tanh()] if layer_norm else [nn.Linear(last, h), nn.Tanh()]
                 last = h
             return nn.Sequential(*layers)
 
@@ -53,17 +60,25 @@ class _MlpExtractor(nn.Module):
 
 
 class ActorCriticPolicy(nn.Module):
-    """SB3 ActorCriticPolicy with the default MlpExtractor (stable_baselines3/common/policies.py)."""
+    """SB3 ActorCriticPolicy with the default MlpExtractor (stable_baselines3/common/policies.py).
 
-    def __init__(self, obs_dim, action_dim=None, nvec=None, net_arch=(64, 64), log_std_init=0.0, ortho_init=True):
+    layer_norm: ``ops.LayerNorm`` before every hidden tanh (SB3's checkpoints have none).  fused_sampling
+    (MultiDiscrete): actions are drawn by ``ops.sample_logits`` from one uniform number each, all dimensions of equal size in one
+    launch -- the same distribution as the default draws, from another use of the random stream."""
+
+    def __init__(self, obs_dim, action_dim=None, nvec=None, net_arch=(64, 64), log_std_init=0.0, ortho_init=True,
+                 layer_norm=False, fused_sampling=False):
         super().__init__()
         if (action_dim is None) == (nvec is None):
             raise ValueError("give action_dim (Box) or nvec (MultiDiscrete)")
+        if fused_sampling and nvec is None:
+            raise ValueError("fused_sampling draws categories: it needs nvec (MultiDiscrete)")
+        self.fused_sampling = bool(fused_sampling)
         self.obs_dim = int(obs_dim)
         self.discrete = nvec is not None
         self.nvec = [int(n) for n in nvec] if self.discrete else None
         self.action_dim = len(self.nvec) if self.discrete else int(action_dim)
-        self.mlp_extractor = _MlpExtractor(self.obs_dim, list(net_arch))
+        self.mlp_extractor = _MlpExtractor(self.obs_dim, list(net_arch), layer_norm)
         lat = self.mlp_extractor.latent_dim
         if self.discrete:
             self.action_net = nn.Linear(lat, sum(self.nvec))
@@ -102,8 +117,29 @@ class ActorCriticPolicy(nn.Module):
         ent = 0.5 + 0.5 * math.log(2 * math.pi) + self.log_std
         return logp.sum(-1), ent.expand_as(head).sum(-1)
 
-    def _sample(self, head, deterministic, generator=None):
+    def action_logits(self, head):
+        """a MultiDiscrete head's logits as [batch, dimensions, categories] views, one for each run of dimensions with
+        equally many categories"""
+        out, o, i = [], 0, 0
+        while i < len(self.nvec):
+            n, m = self.nvec[i], 1
+            while i + m < len(self.nvec) and self.nvec[i + m] == n:
+                m += 1
+            out.append(head[:, o:o + m * n].unflatten(1, (m, n)))
+            o += m * n
+            i += m
+        return out
+
+    def _sample(self, head, deterministic, generator=None, **settings):
         """`generator`: the sampling stream (PPO keeps one per rank); None = torch's global RNG"""
+        if self.discrete and not deterministic and (settings or self.fused_sampling):
+            outs = []
+            for logits in self.action_logits(head):
+                u = torch.rand(logits.shape[:-1], device=head.device, generator=generator)
+                outs.append(ops.sample_logits(logits, u, **settings))
+            # a policy that has become NaN draws -1 throughout: category 0 keeps the actions in range, their
+            # log-probabilities stay NaN
+            return torch.cat(outs, 1).clamp(min=0).to(torch.float32)
         if self.discrete:
             outs, o = [], 0
             for n in self.nvec:
@@ -126,19 +162,43 @@ class ActorCriticPolicy(nn.Module):
         logp, _ = self._log_prob_entropy(head, actions)
         return actions, values, logp
 
-    def evaluate_actions(self, obs, actions):
+    def _evaluate(self, obs, actions):
         head, values = self._dist_params(obs)
         logp, ent = self._log_prob_entropy(head, actions)
-        return values, logp, ent
+        return values, logp, ent, head
+
+    def evaluate_actions(self, obs, actions):
+        return self._evaluate(obs, actions)[:3]
 
     def predict_values(self, obs):
         obs = obs.float()
         return self.value_net(self.mlp_extractor.value_net(obs)).squeeze(-1)
 
     @torch.no_grad()
-    def predict(self, obs, deterministic=True, generator=None):
+    def predict(self, obs, deterministic=True, generator=None, **settings):
+        """`settings` (MultiDiscrete, with deterministic=False): temperature, top_k, top_p, min_p of
+        ``ops.sample_logits`` (numbers)"""
+        if settings and (deterministic or not self.discrete):
+            raise ValueError(f"{', '.join(settings)}: for actions that a MultiDiscrete policy draws (deterministic=False)")
+        unknown = set(settings) - {"temperature", "top_k", "top_p", "min_p"}
+        if unknown:
+            raise TypeError(f"predict() got unexpected settings: {', '.join(sorted(unknown))}")
         head, _ = self._dist_params(obs)
-        return self._sample(head, deterministic, generator)
+        return self._sample(head, deterministic, generator, **settings)
+
+    @torch.no_grad()
+    def top_logits(self, obs, k=None):
+        """what a student of this MultiDiscrete policy learns from: (category indices, logits) of the k largest logits
+        of every action dimension (all of them without k), a pair of [batch, dimensions, k] tensors for each run of
+        equal dimensions (``action_logits``)"""
+        if not self.discrete:
+            raise ValueError("top_logits needs a MultiDiscrete policy")
+        head = self.action_net(self.mlp_extractor.policy_net(obs.float()))
+        out = []
+        for logits in self.action_logits(head):
+            top = logits.topk(min(k or logits.shape[-1], logits.shape[-1], ops.MAX_LISTED), -1)
+            out.append((top.indices, top.values))
+        return out
 
     @classmethod
     def for_env(cls, env, net_arch=(128, 128), **kw):
@@ -168,11 +228,16 @@ def flat_allreduce(tensors, dist, group=None):
 
 class PPO:
     """SB3 PPO (stable_baselines3/ppo/ppo.py) over a FactoryVecEnv; hyperparameters default to SB3's, except
-    n_steps / batch_size (see module docstring)."""
+    n_steps / batch_size (see module docstring).
+
+    teacher: a MultiDiscrete ActorCriticPolicy with the student's nvec.  Every rollout records its distill_top_k
+    largest logits (None: all) at the student's observations, and the update adds distill_coef times
+    ``ops.distill_loss`` at distill_temperature, summed over action dimensions, to the loss."""
 
     def __init__(self, env, policy_kwargs=None, learning_rate=3e-4, n_steps=16, batch_size=8192, n_epochs=10,
                  gamma=0.99, gae_lambda=0.95, clip_range=0.2, ent_coef=0.0, vf_coef=0.5, max_grad_norm=0.5,
-                 normalize_advantage=True, seed=0, dist=None, policy=None):
+                 normalize_advantage=True, seed=0, dist=None, policy=None, teacher=None, distill_coef=1.0,
+                 distill_temperature=1.0, distill_top_k=None):
         self.env = env
         self.device = env.device
         self.dist = dist if (dist is not None and dist.is_available() and dist.is_initialized()) else None
@@ -184,11 +249,21 @@ class PPO:
         if self.dist:  # identical initial weights on every rank
             for p in self.policy.parameters():
                 self.dist.broadcast(p.data, 0)
+        if teacher is not None and not (self.policy.discrete and teacher.discrete and teacher.nvec == self.policy.nvec
+                                        and teacher.obs_dim == self.policy.obs_dim):
+            raise ValueError("teacher: a MultiDiscrete policy with the student's nvec and observations is needed")
+        if distill_top_k is not None and distill_top_k < 1:
+            raise ValueError("distill_top_k is at least 1 (None: every category)")
+        self.teacher = None if teacher is None else teacher.to(self.device)
         self.optimizer = torch.optim.Adam(self.policy.parameters(), lr=learning_rate, eps=1e-5)
         self.hp = dict(learning_rate=learning_rate, n_steps=n_steps, batch_size=batch_size, n_epochs=n_epochs,
                        gamma=gamma, gae_lambda=gae_lambda, clip_range=clip_range, ent_coef=ent_coef, vf_coef=vf_coef,
                        max_grad_norm=max_grad_norm, normalize_advantage=normalize_advantage, seed=seed,
                        world_size=self.world, net_arch=list(pk["net_arch"]))
+        if pk.get("layer_norm"):
+            self.hp["layer_norm"] = True
+        if self.teacher is not None:
+            self.hp.update(distill_coef=distill_coef, distill_temperature=distill_temperature, distill_top_k=distill_top_k)
         # per-rank streams: minibatch permutations, and the rollout's action sampling -- every rank starts from the
         # same broadcast weights (and often identical arenas), so a shared seed would make the ranks' rollouts
         # bit-identical and shrink the effective batch by the world size
@@ -229,6 +304,13 @@ class PPO:
             buf["starts"][t] = self._last_starts
             buf["values"][t] = values
             buf["logp"][t] = logp
+            if self.teacher is not None:
+                for i, (index, logits) in enumerate(self.teacher.top_logits(obs, self.hp["distill_top_k"])):
+                    if t == 0:
+                        buf[f"teacher_index{i}"] = index.new_empty((T, *index.shape))
+                        buf[f"teacher_logits{i}"] = logits.new_empty((T, *logits.shape))
+                    buf[f"teacher_index{i}"][t] = index
+                    buf[f"teacher_logits{i}"][t] = logits
             # Monitor episodes (r, l) of the arenas that ended this step
             ep_r += (env.ep_return * done).sum()
             ep_n += done.sum().to(torch.float64)
@@ -264,7 +346,10 @@ class PPO:
                 if norm:  # the global minibatch's mean / unbiased std (torch.std), reduced behind the forward pass
                     st = torch.stack([adv.sum(), (adv * adv).sum(), torch.tensor(float(len(adv)), device=adv.device)])
                     work = self.dist.all_reduce(st, async_op=True) if self.dist else None
-                values, logp, ent = pol.evaluate_actions(obs, act)
+                if self.teacher is None:
+                    values, logp, ent = pol.evaluate_actions(obs, act)
+                else:
+                    values, logp, ent, head = pol._evaluate(obs, act)
                 if norm:
                     if work is not None:
                         work.wait()
@@ -276,6 +361,11 @@ class PPO:
                 vl = torch.nn.functional.mse_loss(flat["returns"][idx], values)
                 el = -ent.mean()
                 loss = pl + hp["ent_coef"] * el + hp["vf_coef"] * vl
+                if self.teacher is not None:
+                    dl = sum(ops.distill_loss(logits, flat[f"teacher_index{i}"][idx], flat[f"teacher_logits{i}"][idx],
+                                              temperature=hp["distill_temperature"]).sum(1)
+                             for i, logits in enumerate(pol.action_logits(head))).mean()
+                    loss = loss + hp["distill_coef"] * dl
                 self.optimizer.zero_grad(set_to_none=False)
                 loss.backward()
                 if self.dist:  # one fused all-reduce of every gradient, then the mean
@@ -287,6 +377,8 @@ class PPO:
                 self.optimizer.step()
                 last = dict(policy_loss=pl.detach(), value_loss=vl.detach(), entropy_loss=el.detach(),
                             clip_fraction=((ratio - 1).abs() > clip).float().mean().detach())
+                if self.teacher is not None:
+                    last["distill_loss"] = dl.detach()
         return {k: float(v) for k, v in last.items()}
 
     def learn(self, total_timesteps, log_every=1, callback=None):
