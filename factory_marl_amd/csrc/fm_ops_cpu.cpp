@@ -110,7 +110,7 @@ int check_sample(const fm_sample_args* a) {
   if (a->u_dtype != FM_DTYPE_F32 && a->u_dtype != FM_DTYPE_F64) return bad("sample: u_dtype is F32 or F64");
   if (a->rows < 0 || a->cols < 1 || a->cols >= INT32_MAX) return bad("sample: rows >= 0 and 1 <= cols < 2^31 - 1 are needed");
   if (a->stride < 0 || a->mask_stride < 0) return bad("sample: negative row stride");
-  if (!fits(a->rows, a->cols, a->stride) || !fits(a->rows, a->cols, a->mask_stride)) return bad("sample: too many elements");
+  if (!fits(a->rows, a->cols, a->stride) || !fits(a->rows, a->cols, a->mask_stride) || a->rows >> 35) return bad("sample: too many elements");
   if (a->rows > 0 && (!a->logits || !a->u || !a->out)) return bad("sample: logits, u and out are needed");
   if (!aligned(a->logits, type_size(a->dtype)) || !aligned(a->u, type_size(a->u_dtype)) || !aligned(a->out, 8) ||
       !aligned(a->temperature_rows, 4) || !aligned(a->top_p_rows, 4) || !aligned(a->min_p_rows, 4) || !aligned(a->top_k_rows, 4))
