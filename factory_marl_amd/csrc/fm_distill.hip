@@ -2,6 +2,9 @@
 //
 //   loss = T^2 sum over the listed entries of p (log p - log q[index]),  q = softmax(z / T),  p = softmax(teacher / T)
 //   dz_j = grad T (q_j - sum of p over the entries that list j)
+#include <cfloat>
+#include <type_traits>
+
 #include "fm_ops_dev.hpp"
 
 namespace fm {
@@ -14,7 +17,8 @@ struct Teacher {
   const void* logit;
   int64_t logit_stride;
   int index64, logit_type, k, cols;
-  float inv_t;
+  float temperature, c;  // c: log2(e) / T
+  double inv_t, t2;
 };
 
 __device__ __forceinline__ int64_t index_at(const Teacher& t, int64_t row, int i) {
@@ -25,6 +29,9 @@ __device__ __forceinline__ float logit_at(const Teacher& t, int64_t row, int i) 
   const int64_t o = row * t.logit_stride + i;
   return t.logit_type == FM_DTYPE_F32 ? ((const float*)t.logit)[o] : t.logit_type == FM_DTYPE_F16 ? (float)((const f16*)t.logit)[o] : (float)((const bf16*)t.logit)[o];
 }
+
+// exp2 of at most 0; the hardware's, to one unit in the last place
+__device__ __forceinline__ float exp2_neg(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // The row's entries into LDS: at[i] (-1: not listed) and p[i].  Returns 1, 0 where none is listed, NaN where an
 // index is too large or a logit NaN or +inf.  top, total: the teacher's largest logit and its sum of exp.
@@ -42,7 +49,7 @@ __device__ float load_teacher(const Teacher& t, int64_t row, int* at, float* p, 
   top = block_max<NT>(m, buf);
   wrong = block_max<NT>(wrong, buf + NT / 64);
   for (int i = threadIdx.x; i < t.k; i += NT) {
-    const float e = at[i] < 0 ? 0.0f : expf((p[i] - top) * t.inv_t);
+    const float e = at[i] < 0 ? 0.0f : exp2_neg((p[i] - top) * t.c);
     p[i] = e;
     s += e;
   }
@@ -53,87 +60,366 @@ __device__ float load_teacher(const Teacher& t, int64_t row, int* at, float* p, 
   return wrong > 0 ? NAN : total > 0 ? 1.0f : 0.0f;
 }
 
-template <typename T>
-__global__ __launch_bounds__(NT) void distill_fwd(const T* z, int64_t stride, Teacher t, float temperature, float* loss, float* stats, int64_t rows) {
-  __shared__ int at[FM_DISTILL_MAX_K];
-  __shared__ float p[FM_DISTILL_MAX_K];
-  __shared__ float buf[5 * (NT / 64)];
-  __shared__ double dbuf[NT / 64];
-  for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
+// Largest logit and sum of exp((z - largest) / T), one pass: the sum is scaled down where a larger logit comes along.
+// The difference comes before the scaling: both may be near the type's lowest value.
+struct Softmax {
+  float m = -FLT_MAX, s = 0;
+  template <int N>
+  __device__ __forceinline__ void add(const float* v, float c) {
+    float mx = v[0];
+#pragma unroll
+    for (int i = 1; i < N; i++) mx = fmaxf(mx, v[i]);
+    if (mx > m) {
+      s *= exp2_neg((m - mx) * c);
+      m = mx;
+    }
+#pragma unroll
+    for (int i = 0; i < N; i++) s += exp2_neg((v[i] - m) * c);
+  }
+  __device__ __forceinline__ void rescale(float top, float c) {
+    s *= exp2_neg((m - top) * c);
+    m = top;
+  }
+};
+
+// f(first column, N logits as floats) over columns [from, to) by `threads` threads, of which this is `t`: U 16-byte
+// loads on their way at a time, from any element on; g(column, logit) for the elements that are left
+template <int U, typename T, typename F, typename G>
+__device__ __forceinline__ void each(const T* z, int from, int to, int t, int threads, F&& f, G&& g) {
+  constexpr int N = 16 / (int)sizeof(T);
+  const int vectors = (to - from) / N;
+  int i = t;
+  for (; i + (U - 1) * threads < vectors; i += U * threads) {
+    T v[U][N];
+#pragma unroll
+    for (int u = 0; u < U; u++) __builtin_memcpy(v[u], z + from + (i + u * threads) * N, 16);
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      float x[N];
+#pragma unroll
+      for (int n = 0; n < N; n++) x[n] = to_f32(v[u][n]);
+      f(from + (i + u * threads) * N, x);
+    }
+  }
+  for (; i < vectors; i += threads) {
+    T v[N];
+    __builtin_memcpy(v, z + from + i * N, 16);
+    float x[N];
+#pragma unroll
+    for (int n = 0; n < N; n++) x[n] = to_f32(v[n]);
+    f(from + i * N, x);
+  }
+  const int c = from + vectors * N + t;
+  if (c < to) g(c, to_f32(z[c]));
+}
+
+// ---------------------------------------------------------------------------------------------- short rows and lists
+// G lanes a row, k <= G: each lane has an entry of the list, and one column (or, WIDE with G = 64, vectors of them).
+struct Entry {
+  int at;  // its column; -1: not listed
+  float p, logit, top, total, mass;
+};
+template <int G>
+__device__ __forceinline__ Entry entry_of(const Teacher& t, int64_t row, int j, uint64_t group) {
+  Entry e;
+  const int64_t at = j < t.k ? index_at(t, row, j) : -1;
+  e.logit = at < 0 ? -INFINITY : logit_at(t, row, j);
+  const bool wrong = (__ballot(at >= t.cols || !(e.logit < INFINITY)) & group) != 0;
+  e.at = e.logit == -INFINITY || at >= t.cols ? -1 : (int)at;
+  e.top = group_max<G>(e.logit);
+  const float x = e.at < 0 ? 0.0f : exp2_neg((e.logit - e.top) * t.c);
+  e.total = group_sum<G>(x);
+  e.p = x / e.total;
+  e.mass = wrong ? NAN : e.total > 0 ? 1.0f : 0.0f;
+  return e;
+}
+
+template <typename T, int G, bool WIDE>
+__device__ __forceinline__ Softmax softmax_of(const T* zr, int j, const Teacher& t) {
+  Softmax q;
+  if (WIDE) {
+    each<2>(zr, 0, t.cols, j, 64, [&](int, const float* v) { q.add<16 / (int)sizeof(T)>(v, t.c); }, [&](int, float v) { q.add<1>(&v, t.c); });
+  } else if (j < t.cols) {
+    const float v = to_f32(zr[j]);
+    q.add<1>(&v, t.c);
+  }
+  q.rescale(group_max<G>(q.m), t.c);
+  q.s = group_sum<G>(q.s);
+  return q;
+}
+
+__device__ __forceinline__ double term_of(float p, float teacher, float top, double log_total, float z, float m, double log_s, const Teacher& t) {
+  return (double)p * ((((double)teacher - top) - ((double)z - m)) * t.inv_t - log_total + log_s);
+}
+
+template <typename T, int G, bool WIDE>
+__global__ __launch_bounds__(NT) void distill_fwd_group(const T* z, int64_t stride, Teacher t, float* loss, float* stats, int64_t rows) {
+  const int lane = threadIdx.x & 63, j = lane & (G - 1);
+  const uint64_t group = (G == 64 ? ~0ull : (1ull << G) - 1) << (lane - j);
+  for (int64_t first = (int64_t)blockIdx.x * (NT / G); first < rows; first += (int64_t)gridDim.x * (NT / G)) {
+    const int64_t row = first + threadIdx.x / G, r = row < rows ? row : rows - 1;
     const T* zr = z + r * stride;
-    float m = -INFINITY;
-    for (int c = threadIdx.x; c < t.cols; c += NT) m = fmaxf(m, to_f32(zr[c]));
-    m = block_max<NT>(m, buf + 3 * (NT / 64));
-    float s = 0;
-    for (int c = threadIdx.x; c < t.cols; c += NT) {
-      const float v = to_f32(zr[c]);
-      s += v == -INFINITY ? 0.0f : expf((v - m) * t.inv_t);
-    }
-    s = block_sum<NT>(s, buf + 4 * (NT / 64));
-    float top, total;
-    const float mass = load_teacher(t, r, at, p, buf, top, total);
-    const double log_s = log((double)s), log_total = log((double)total);
+    const Entry e = entry_of<G>(t, r, j, group);
+    const Softmax q = softmax_of<T, G, WIDE>(zr, j, t);
     double sum = 0;
-    for (int i = threadIdx.x; i < t.k; i += NT)
-      if (p[i] > 0) {
-        const float v = to_f32(zr[at[i]]);
-        const double logp = ((double)logit_at(t, r, i) - top) * t.inv_t - log_total;
-        sum += (double)p[i] * (logp - ((double)v - m) * t.inv_t + log_s);
-      }
-    sum = block_sum<NT>(sum, dbuf);
-    if (threadIdx.x == 0) {
-      loss[r] = mass != mass ? mass : mass == 0 ? 0.0f : (float)((double)temperature * temperature * sum);
-      if (stats) {
-        stats[2 * r] = m;
-        stats[2 * r + 1] = s;
-      }
+    if (e.p > 0) sum = term_of(e.p, e.logit, e.top, log((double)e.total), to_f32(zr[e.at]), q.m, log((double)q.s), t);
+    sum = group_sum<G>(sum);
+    if (j || row >= rows) continue;
+    loss[row] = e.mass != e.mass ? e.mass : e.mass == 0 ? 0.0f : (float)(t.t2 * sum);
+    if (stats) {
+      stats[2 * row] = q.m;
+      stats[2 * row + 1] = q.s;
     }
-    __syncthreads();
   }
 }
 
-// dlogits of one row a block: everything first as if nothing were listed, then the listed places again, each with all
-// of the entries that list it (whoever writes the same place writes the same value).
-template <typename T>
-__global__ __launch_bounds__(NT) void distill_bwd(const T* z, int64_t stride, Teacher t, float temperature, const float* stats, const float* grad,
-                                                  int64_t grad_stride, T* dz, int64_t rows) {
-  __shared__ int at[FM_DISTILL_MAX_K];
-  __shared__ float p[FM_DISTILL_MAX_K];
-  __shared__ float buf[3 * (NT / 64)];
-  for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
+template <typename T, int G, bool WIDE>
+__global__ __launch_bounds__(NT) void distill_bwd_group(const T* z, int64_t stride, Teacher t, const float* stats, const float* grad, int64_t grad_stride,
+                                                        T* dz, int64_t rows) {
+  const int lane = threadIdx.x & 63, j = lane & (G - 1), base = lane - j;
+  const uint64_t group = (G == 64 ? ~0ull : (1ull << G) - 1) << base;
+  for (int64_t first = (int64_t)blockIdx.x * (NT / G); first < rows; first += (int64_t)gridDim.x * (NT / G)) {
+    const int64_t row = first + threadIdx.x / G, r = row < rows ? row : rows - 1;
     const T* zr = z + r * stride;
     T* dr = dz + r * (int64_t)t.cols;
-    float top, total;
-    const float mass = load_teacher(t, r, at, p, buf, top, total);
-    const float m = stats[2 * r], inv = 1.0f / stats[2 * r + 1], scale = mass == 0 ? 0.0f : grad[r * grad_stride] * temperature;
-    for (int c = threadIdx.x; c < t.cols; c += NT) {
-      const float v = to_f32(zr[c]);
-      const float q = v == -INFINITY ? 0.0f * inv : expf((v - m) * t.inv_t) * inv;
-      dr[c] = from_f32<T>(mass == 0 ? 0.0f : mass * scale * q);
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < t.k; i += NT) {
-      const int j = at[i];
-      if (j < 0 || mass == 0) continue;
+    const Entry e = entry_of<G>(t, r, j, group);
+    const float m = stats[2 * r], inv = 1.0f / stats[2 * r + 1], scale = e.mass == 0 ? 0.0f : e.mass * grad[r * grad_stride] * t.temperature;
+    auto part = [&](float v, float listed) { return e.mass == 0 ? 0.0f : scale * (exp2_neg((v - m) * t.c) * inv - listed); };
+    // what the row's entries list at column c of each lane's own
+    auto listed_at = [&](int c) {
       float listed = 0;
-      for (int n = 0; n < t.k; n++) listed += at[n] == j ? p[n] : 0.0f;
-      const float v = to_f32(zr[j]);
-      const float q = v == -INFINITY ? 0.0f * inv : expf((v - m) * t.inv_t) * inv;
-      dr[j] = from_f32<T>(mass * scale * (q - listed));
+      for (int i = 0; i < t.k; i++) {
+        const int at = __shfl(e.at, base + i);
+        const float p = __shfl(e.p, base + i);
+        listed += at == c ? p : 0.0f;
+      }
+      return listed;
+    };
+    if (!WIDE) {
+      const float listed = listed_at(j);
+      if (j < t.cols && row < rows) dr[j] = from_f32<T>(part(to_f32(zr[j]), listed));
+      continue;
     }
-    __syncthreads();
+    if (row < rows) {  // the same for the whole wave
+      constexpr int N = 16 / (int)sizeof(T);
+      each<2>(
+          zr, 0, t.cols, j, 64,
+          [&](int c, const float* v) {
+            T o[N];
+#pragma unroll
+            for (int n = 0; n < N; n++) o[n] = from_f32<T>(part(v[n], 0.0f));
+            __builtin_memcpy(dr + c, o, 16);
+          },
+          [&](int c, float v) { dr[c] = from_f32<T>(part(v, 0.0f)); });
+      const float listed = listed_at(e.at);
+      wave_sync();
+      // the listed columns again: whoever lists the same one writes the same value
+      if (e.at >= 0 && e.mass == 1) dr[e.at] = from_f32<T>(part(to_f32(zr[e.at]), listed));
+    }
   }
 }
 
+// ---------------------------------------------------------------------------------------------- long rows and lists
+// Columns [from, to) of split y of a row: of vectors, so that each starts where the loads do.
+template <typename T>
+__device__ __forceinline__ void split_of(int cols, int y, int splits, int& from, int& to) {
+  constexpr int N = 16 / (int)sizeof(T);
+  const int each = ((cols + splits - 1) / splits + N - 1) / N * N;
+  from = min(y * each, cols);
+  to = min(from + each, cols);
+}
+
+template <typename T>
+__device__ __forceinline__ Softmax block_softmax(const T* zr, int from, int to, const Teacher& t, float* buf) {
+  Softmax q;
+  each<4>(zr, from, to, threadIdx.x, NT, [&](int, const float* v) { q.add<16 / (int)sizeof(T)>(v, t.c); }, [&](int, float v) { q.add<1>(&v, t.c); });
+  q.rescale(block_max<NT>(q.m, buf), t.c);
+  q.s = block_sum<NT>(q.s, buf + NT / 64);
+  return q;
+}
+
+template <typename T>
+__device__ __forceinline__ void write_loss(const T* zr, const Teacher& t, int64_t r, const Softmax& q, float* loss, float* stats, int* at, float* p, float* buf,
+                                           double* dbuf) {
+  float top, total;
+  const float mass = load_teacher(t, r, at, p, buf, top, total);
+  const double log_s = log((double)q.s), log_total = log((double)total);
+  double sum = 0;
+  for (int i = threadIdx.x; i < t.k; i += NT)
+    if (p[i] > 0) sum += term_of(p[i], logit_at(t, r, i), top, log_total, to_f32(zr[at[i]]), q.m, log_s, t);
+  sum = block_sum<NT>(sum, dbuf);
+  if (threadIdx.x) return;
+  loss[r] = mass != mass ? mass : mass == 0 ? 0.0f : (float)(t.t2 * sum);
+  if (stats) {
+    stats[2 * r] = q.m;
+    stats[2 * r + 1] = q.s;
+  }
+}
+
+// a block a row
+template <typename T>
+__global__ __launch_bounds__(NT) void distill_fwd(const T* z, int64_t stride, Teacher t, float* loss, float* stats, int64_t rows) {
+  __shared__ int at[FM_DISTILL_MAX_K];
+  __shared__ float p[FM_DISTILL_MAX_K], buf[5 * (NT / 64)];
+  __shared__ double dbuf[NT / 64];
+  const int64_t r = blockIdx.x + (int64_t)gridDim.x * blockIdx.y;
+  if (r >= rows) return;
+  const Softmax q = block_softmax(z + r * stride, 0, t.cols, t, buf + 3 * (NT / 64));
+  write_loss(z + r * stride, t, r, q, loss, stats, at, p, buf, dbuf);
+}
+
+// Few rows: a block for each of a row's splits, whose softmax goes to part [rows][splits][2], then a block a row.
+template <typename T>
+__global__ __launch_bounds__(NT) void distill_fwd_split(const T* z, int64_t stride, Teacher t, float* part) {
+  __shared__ float buf[2 * (NT / 64)];
+  int from, to;
+  split_of<T>(t.cols, blockIdx.x, gridDim.x, from, to);
+  const Softmax q = block_softmax(z + (int64_t)blockIdx.y * stride, from, to, t, buf);
+  if (threadIdx.x == 0) {
+    float* o = part + 2 * ((int64_t)blockIdx.y * gridDim.x + blockIdx.x);
+    o[0] = q.m;
+    o[1] = q.s;
+  }
+}
+template <typename T>
+__global__ __launch_bounds__(NT) void distill_fwd_join(const T* z, int64_t stride, Teacher t, const float* part, int splits, float* loss, float* stats) {
+  __shared__ int at[FM_DISTILL_MAX_K];
+  __shared__ float p[FM_DISTILL_MAX_K], buf[5 * (NT / 64)];
+  __shared__ double dbuf[NT / 64];
+  const int64_t r = blockIdx.x;
+  Softmax q;
+  if ((int)threadIdx.x < splits) {  // at most 64: every wave joins them
+    q.m = part[2 * (r * splits + threadIdx.x)];
+    q.s = part[2 * (r * splits + threadIdx.x) + 1];
+  }
+  q.rescale(block_max<NT>(q.m, buf + 3 * (NT / 64)), t.c);
+  q.s = block_sum<NT>(q.s, buf + 4 * (NT / 64));
+  write_loss(z + r * stride, t, r, q, loss, stats, at, p, buf, dbuf);
+}
+
+// dlogits of a split of a row a block: everything first as if nothing were listed, then the listed columns of the split
+// again, each with all of the entries that list it (whoever lists the same one writes the same value).
+template <typename T>
+__global__ __launch_bounds__(NT) void distill_bwd(const T* z, int64_t stride, Teacher t, const float* stats, const float* grad, int64_t grad_stride, T* dz,
+                                                  int64_t rows, int splits) {
+  __shared__ int at[FM_DISTILL_MAX_K];
+  __shared__ float p[FM_DISTILL_MAX_K], buf[3 * (NT / 64)];
+  const int64_t b = blockIdx.x + (int64_t)gridDim.x * blockIdx.y, r = b / splits;
+  if (r >= rows) return;
+  const T* zr = z + r * stride;
+  T* dr = dz + r * (int64_t)t.cols;
+  int from, to;
+  split_of<T>(t.cols, (int)(b - r * splits), splits, from, to);
+  float top, total;
+  const float mass = load_teacher(t, r, at, p, buf, top, total);
+  const float m = stats[2 * r], inv = 1.0f / stats[2 * r + 1], scale = mass == 0 ? 0.0f : mass * grad[r * grad_stride] * t.temperature;
+  auto part = [&](float v, float listed) { return mass == 0 ? 0.0f : scale * (exp2_neg((v - m) * t.c) * inv - listed); };
+  constexpr int N = 16 / (int)sizeof(T);
+  each<4>(
+      zr, from, to, threadIdx.x, NT,
+      [&](int c, const float* v) {
+        T o[N];
+#pragma unroll
+        for (int n = 0; n < N; n++) o[n] = from_f32<T>(part(v[n], 0.0f));
+        __builtin_memcpy(dr + c, o, 16);
+      },
+      [&](int c, float v) { dr[c] = from_f32<T>(part(v, 0.0f)); });
+  if (mass != 1) return;
+  __syncthreads();
+  for (int i = threadIdx.x; i < t.k; i += NT) {
+    const int c = at[i];
+    if (c < from || c >= to) continue;
+    float listed = 0;
+    for (int n = 0; n < t.k; n++) listed += at[n] == c ? p[n] : 0.0f;
+    dr[c] = from_f32<T>(part(to_f32(zr[c]), listed));
+  }
+}
+
+// ---------------------------------------------------------------------------------------------- the choice
 Teacher teacher_of(const fm_distill_args& a) {
-  return Teacher{a.index, a.index_stride, a.teacher, a.teacher_stride, a.index_dtype == FM_DTYPE_I64, a.teacher_dtype, (int)a.k, (int)a.cols, (float)(1.0 / a.temperature)};
+  return Teacher{a.index, a.index_stride, a.teacher, a.teacher_stride, a.index_dtype == FM_DTYPE_I64, a.teacher_dtype, (int)a.k, (int)a.cols,
+                 (float)a.temperature, (float)(1.4426950408889634 / a.temperature), 1.0 / a.temperature, a.temperature * a.temperature};
+}
+
+// splits of a row in the forward pass: where there are fewer rows than fill the chip (4 blocks a CU), of 4096 columns or more
+int splits_of(int64_t rows, int64_t cols) {
+  if (rows < 1 || rows >= 1024) return 1;
+  const int64_t wanted = 1024 / rows, most = cols / 4096;
+  const int64_t n = wanted < most ? wanted : most;
+  return (int)(n < 1 ? 1 : n > 64 ? 64 : n);
+}
+
+// f(lanes, wide) for rows and lists that a group of lanes holds; false for longer ones
+template <typename F>
+bool with_group(int64_t cols, int64_t k, F&& f) {
+  if (k > 64 || cols > 2048) return false;
+#define GROUP(g, w) f(std::integral_constant<int, g>(), std::integral_constant<bool, w>())
+  const int64_t n = cols > k ? cols : k;
+  if (n <= 2)
+    GROUP(2, false);
+  else if (n <= 4)
+    GROUP(4, false);
+  else if (n <= 8)
+    GROUP(8, false);
+  else if (n <= 16)
+    GROUP(16, false);
+  else if (n <= 32)
+    GROUP(32, false);
+  else if (n <= 64)
+    GROUP(64, false);
+  else
+    GROUP(64, true);
+#undef GROUP
+  return true;
+}
+
+// n blocks as a grid that holds any number of them
+dim3 grid_of(int64_t n) { return dim3((unsigned)(n < (1 << 20) ? n : 1 << 20), (unsigned)((n + (1 << 20) - 1) >> 20)); }
+
+template <typename T>
+void forward(const fm_distill_args& a) {
+  hipStream_t st = (hipStream_t)a.stream;
+  const Teacher t = teacher_of(a);
+  const T* z = (const T*)a.logits;
+  if (with_group(a.cols, a.k, [&](auto g, auto w) {
+        const int64_t n = (a.rows + NT / g - 1) / (NT / g);
+        distill_fwd_group<T, decltype(g)::value, decltype(w)::value><<<(int)(n < (1 << 20) ? n : 1 << 20), NT, 0, st>>>(z, a.stride, t, a.loss, a.stats, a.rows);
+      }))
+    return;
+  const int splits = splits_of(a.rows, a.cols);
+  if (splits > 1) {
+    distill_fwd_split<T><<<dim3(splits, (int)a.rows), NT, 0, st>>>(z, a.stride, t, (float*)a.workspace);
+    distill_fwd_join<T><<<(int)a.rows, NT, 0, st>>>(z, a.stride, t, (const float*)a.workspace, splits, a.loss, a.stats);
+  } else {
+    distill_fwd<T><<<grid_of(a.rows), NT, 0, st>>>(z, a.stride, t, a.loss, a.stats, a.rows);
+  }
+}
+
+template <typename T>
+void backward(const fm_distill_args& a) {
+  hipStream_t st = (hipStream_t)a.stream;
+  const Teacher t = teacher_of(a);
+  const T* z = (const T*)a.logits;
+  if (with_group(a.cols, a.k, [&](auto g, auto w) {
+        const int64_t n = (a.rows + NT / g - 1) / (NT / g);
+        distill_bwd_group<T, decltype(g)::value, decltype(w)::value>
+            <<<(int)(n < (1 << 20) ? n : 1 << 20), NT, 0, st>>>(z, a.stride, t, a.stats, a.grad, a.grad_stride, (T*)a.dlogits, a.rows);
+      }))
+    return;
+  // a block for every 32768 columns (the list is read again for each), for fewer where that leaves CUs without work
+  int64_t splits = (a.cols + 32767) / 32768;
+  if (a.rows * splits < 1024) splits = splits_of(a.rows, a.cols) > splits ? splits_of(a.rows, a.cols) : splits;
+  distill_bwd<T><<<grid_of(a.rows * splits), NT, 0, st>>>(z, a.stride, t, a.stats, a.grad, a.grad_stride, (T*)a.dlogits, a.rows, (int)splits);
 }
 }  // namespace
 }  // namespace fm
 
 using namespace fm;
 extern "C" {
-int64_t fm_distill_workspace(int64_t rows, int64_t cols) { return 0; }
+int64_t fm_distill_workspace(int64_t rows, int64_t cols) {
+  const int n = splits_of(rows, cols);
+  return n > 1 ? rows * n * 8 : 0;
+}
 
 int fm_distill_forward(const fm_distill_args* a) {
   return guarded([&] {
@@ -144,12 +430,7 @@ int fm_distill_forward(const fm_distill_args* a) {
       return FM_OK;
     }
     OnDevice on(a->device);
-    if (on.err == hipSuccess)
-      with_type(a->dtype, [&](auto tag) {
-        typedef typename decltype(tag)::type T;
-        distill_fwd<T><<<(int)(a->rows < (1 << 20) ? a->rows : 1 << 20), NT, 0, (hipStream_t)a->stream>>>(
-            (const T*)a->logits, a->stride, teacher_of(*a), (float)a->temperature, a->loss, a->stats, a->rows);
-      });
+    if (on.err == hipSuccess) with_type(a->dtype, [&](auto tag) { forward<typename decltype(tag)::type>(*a); });
     return on.status("distill");
   });
 }
@@ -163,12 +444,7 @@ int fm_distill_backward(const fm_distill_args* a) {
       return FM_OK;
     }
     OnDevice on(a->device);
-    if (on.err == hipSuccess)
-      with_type(a->dtype, [&](auto tag) {
-        typedef typename decltype(tag)::type T;
-        distill_bwd<T><<<(int)(a->rows < (1 << 20) ? a->rows : 1 << 20), NT, 0, (hipStream_t)a->stream>>>(
-            (const T*)a->logits, a->stride, teacher_of(*a), (float)a->temperature, a->stats, a->grad, a->grad_stride, (T*)a->dlogits, a->rows);
-      });
+    if (on.err == hipSuccess) with_type(a->dtype, [&](auto tag) { backward<typename decltype(tag)::type>(*a); });
     return on.status("distill backward");
   });
 }

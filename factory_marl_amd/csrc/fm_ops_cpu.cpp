@@ -136,6 +136,7 @@ int check_distill(const fm_distill_args* a, bool backward) {
   if (!fits(a->rows, a->cols, a->stride) || !fits(a->rows, a->k, a->index_stride) || !fits(a->rows, a->k, a->teacher_stride) ||
       (backward && !fits(a->rows, 1, a->grad_stride)))
     return bad("distill: too many elements");
+  if (a->rows >> 35) return bad("distill: too many rows");
   if (!(a->temperature > 0) || !(a->temperature >= 1e-30 && a->temperature <= 1e30)) return bad("distill: temperature is positive and within 1e-30 .. 1e30");
   if (a->rows > 0 && (!a->logits || !a->index || !a->teacher)) return bad("distill: logits, index and teacher are needed");
   if (a->rows > 0 && !backward && !a->loss) return bad("distill: loss is NULL");

@@ -20,6 +20,13 @@ __device__ __forceinline__ T from_f32(float v) {
   return (T)v;  // to the nearest, ties to even
 }
 
+// what a wave's lanes wrote before is there for its other lanes after
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 // sums and maxima over groups of G lanes (a power of two up to 64); every lane gets the result, the order is fixed
 template <int G, typename V>
 __device__ __forceinline__ V group_sum(V v) {

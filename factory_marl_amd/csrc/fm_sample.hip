@@ -209,12 +209,6 @@ struct List {
   int at;
 };
 
-__device__ __forceinline__ void wave_sync() {
-  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-  __builtin_amdgcn_wave_barrier();
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-}
-
 // Sorts the first n places (the larger first) and sums their weights.  Bitonic: pairs that are at most 64 apart stay
 // within the 128 places of one wave, and need no barrier.  A place of 0 is none.
 template <int NT, int LN>
