@@ -157,15 +157,18 @@ __device__ __forceinline__ float own_sum(int skip, F&& f) {
 // sum over the TPR threads of a row; `buf` holds a value of each of the block's waves
 template <int TPR>
 __device__ __forceinline__ float row_sum(float v, float* buf) {
-  if (TPR <= 64) return group_sum<TPR>(v);
-  v = group_sum<64>(v);
-  if ((threadIdx.x & 63) == 0) buf[threadIdx.x >> 6] = v;
-  __syncthreads();
-  const float* own = buf + threadIdx.x / TPR * (TPR / 64);
-  float s = own[0];
+  if constexpr (TPR <= 64) {
+    return group_sum<TPR>(v);
+  } else {
+    v = group_sum<64>(v);
+    if ((threadIdx.x & 63) == 0) buf[threadIdx.x >> 6] = v;
+    __syncthreads();
+    const float* own = buf + threadIdx.x / TPR * (TPR / 64);
+    float s = own[0];
 #pragma unroll
-  for (int i = 1; i < TPR / 64; i++) s += own[i];
-  return s;
+    for (int i = 1; i < TPR / 64; i++) s += own[i];
+    return s;
+  }
 }
 
 template <typename T, typename P, int NT_, int TPR, int V, int N>

@@ -27,17 +27,83 @@ __device__ __forceinline__ void wave_sync() {
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
-// sums and maxima over groups of G lanes (a power of two up to 64); every lane gets the result, the order is fixed
-template <int G, typename V>
-__device__ __forceinline__ V group_sum(V v) {
+// Exchanges between lanes without LDS: within rows of 16 lanes by data-parallel moves, between them by the row and half swaps.
+// A value of 4 or 8 bytes goes a word at a time.
+template <int CTRL, int ROWS = 0xf>
+__device__ __forceinline__ uint32_t move_word(uint32_t v) {  // lanes that nothing comes to get 0
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, true);
+}
+template <int M>
+__device__ __forceinline__ uint32_t xor_word(uint32_t v) {  // the word of lane number ^ M
+  if constexpr (M == 1) {
+    return move_word<0xB1>(v);  // quads: 1 0 3 2
+  } else if constexpr (M == 2) {
+    return move_word<0x4E>(v);  // quads: 2 3 0 1
+  } else if constexpr (M == 4) {
+    return move_word<0x141>(move_word<0x1B>(v));  // quads reversed (^ 3), then eights (^ 7)
+  } else if constexpr (M == 8) {
+    return move_word<0x140>(move_word<0x141>(v));  // eights reversed (^ 7), then rows (^ 15)
+  } else if constexpr (M == 16) {
+    const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);  // [0] even rows' words twice, [1] odd rows'
+    return threadIdx.x & 16 ? r[0] : r[1];
+  } else {
+    static_assert(M == 32, "");
+    const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);  // [0] the lower half's words twice, [1] the upper's
+    return threadIdx.x & 32 ? r[0] : r[1];
+  }
+}
+template <typename V, typename F>
+__device__ __forceinline__ V by_words(V v, F&& f) {
+  static_assert(sizeof(V) == 4 || sizeof(V) == 8, "");
+  uint32_t w[sizeof(V) / 4];
+  __builtin_memcpy(w, &v, sizeof(V));
 #pragma unroll
-  for (int m = G / 2; m; m >>= 1) v += __shfl_xor(v, m);
+  for (unsigned i = 0; i < sizeof(V) / 4; i++) w[i] = f(w[i]);
+  __builtin_memcpy(&v, w, sizeof(V));
   return v;
 }
-template <int G>
+template <int M, typename V>
+__device__ __forceinline__ V lane_xor(V v) {
+  return by_words(v, [](uint32_t w) { return xor_word<M>(w); });
+}
+
+// sums and maxima over groups of G lanes (a power of two up to 64); every lane gets the result, the order is fixed
+template <int G, int M = 1, typename V>
+__device__ __forceinline__ V group_sum(V v) {
+  if constexpr (M < G)
+    return group_sum<G, 2 * M>(v + lane_xor<M>(v));
+  else
+    return v;
+}
+template <int G, int M = 1>
 __device__ __forceinline__ float group_max(float v) {
-#pragma unroll
-  for (int m = G / 2; m; m >>= 1) v = fmaxf(v, __shfl_xor(v, m));
+  if constexpr (M < G)
+    return group_max<G, 2 * M>(fmaxf(v, lane_xor<M>(v)));
+  else
+    return v;
+}
+// sum over this lane and the ones before it, of G; j: the lane's number among them
+template <int G, typename V>
+__device__ __forceinline__ V sum_lanes(V v, int j) {
+  if constexpr (G > 1) {
+    const V q = by_words(v, [](uint32_t w) { return move_word<0x111>(w); });
+    if (j >= 1) v += q;
+  }
+  if constexpr (G > 2) {
+    const V q = by_words(v, [](uint32_t w) { return move_word<0x112>(w); });
+    if (j >= 2) v += q;
+  }
+  if constexpr (G > 4) {
+    const V q = by_words(v, [](uint32_t w) { return move_word<0x114>(w); });
+    if (j >= 4) v += q;
+  }
+  if constexpr (G > 8) {
+    const V q = by_words(v, [](uint32_t w) { return move_word<0x118>(w); });
+    if (j >= 8) v += q;
+  }
+  // the last lane's of the row before to rows 1 and 3, then of the lower half to rows 2 and 3
+  if constexpr (G > 16) v += by_words(v, [](uint32_t w) { return move_word<0x142, 0xa>(w); });
+  if constexpr (G > 32) v += by_words(v, [](uint32_t w) { return move_word<0x143, 0xc>(w); });
   return v;
 }
 

@@ -9,8 +9,11 @@
 // Weights are exp((logit - largest) / T) in multiples of 2^-s of the largest's, as 64-bit integers: sums are exact,
 // so no result depends on the order in which a launch happens to add, and a border that lies 2^-45 of the row's
 // weight away is still told apart (fp32 sums over 10^5 categories lose 2^-20 and would draw another category).
+#include <type_traits>
+
 #include "fm_ops_dev.hpp"
 
+#define GLOBAL __attribute__((address_space(1)))
 namespace fm {
 namespace {
 
@@ -38,7 +41,7 @@ __device__ __forceinline__ Row row_settings(const Settings& a, int64_t r) {
   o.u = a.u64 ? ((const double*)a.u)[r] : (double)((const float*)a.u)[r];
   o.nan = t != t || o.min_p != o.min_p || o.top_p != o.top_p || o.u != o.u;
   o.greedy = t <= 0;
-  o.inv_t = 1.0 / t;
+  o.inv_t = fmin(1.0 / t, 1e290);
   o.one = (double)(1ull << a.shift);
   o.min_w = ldexp(fmin(o.min_p, 1.0), a.shift);
   return o;
@@ -50,16 +53,24 @@ __device__ __forceinline__ double uniform(double v) {
   return __longlong_as_double((long long)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(b >> 32)) << 32 |
                                           (uint32_t)__builtin_amdgcn_readfirstlane((int)b)));
 }
-__device__ __forceinline__ Row block_settings(const Settings& a, int64_t r) {
-  Row o = row_settings(a, r);
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ float uniform(float v) { return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(v))); }
+template <typename V>
+__device__ __forceinline__ const GLOBAL V* uniform(const V* v) {
+  const uint64_t b = (uint64_t)v;
+  return (const GLOBAL V*)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(b >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((int)b));
+}
+__device__ __forceinline__ Row uniform(Row o) {
   o.inv_t = uniform(o.inv_t);
   o.top_p = uniform(o.top_p);
   o.min_p = uniform(o.min_p);
   o.min_w = uniform(o.min_w);
   o.u = uniform(o.u);
   o.one = uniform(o.one);
+  o.top_k = ((int64_t)uniform((int)(o.top_k >> 32)) << 32) | (uint32_t)uniform((int)o.top_k);
   return o;
 }
+
 
 // ascending as the floats; -0 and +0 are the same
 __device__ __forceinline__ uint32_t key_of(float v) {
@@ -109,46 +120,78 @@ __device__ __forceinline__ uint64_t border_of(double p, uint64_t sum) {
   return t <= 1 ? 0 : t >= (double)sum ? sum - 1 : (uint64_t)t - 1;
 }
 
-// The row's logits: `each` calls f(column, logit) for every category, with -inf where it is barred.  16-byte loads
-// from any element on, U of them on their way at a time; f is called for one after the other (`ordered`: the weights of
-// several at once would spill registers).
+// The row's logits, -inf where a category is barred.  The pointers say that they are to global memory, also in functions of
+// their own.
+typedef uint32_t Vec16 __attribute__((ext_vector_type(4), aligned(1)));
+typedef uint32_t Vec8 __attribute__((ext_vector_type(2), aligned(1)));
+typedef uint32_t Vec4 __attribute__((aligned(1)));
+
 template <typename T, bool MASKED>
 struct Source {
-  const T* z;
-  const uint8_t* mask;
+  static constexpr int N = 16 / (int)sizeof(T);
+  const GLOBAL T* z;
+  const GLOBAL uint8_t* mask;
   int cols;
 
-  template <int NT, int U, bool ORDERED, typename F>
-  __device__ __forceinline__ void each(F&& f) const {
-    constexpr int N = 16 / (int)sizeof(T);
-    const int vectors = cols / N;
-    for (int i = threadIdx.x; i < vectors; i += NT * U) {
-      T v[U][N];
-      uint8_t m[U][N];
+  __device__ __forceinline__ float operator()(int c) const { return MASKED && !mask[c] ? -INFINITY : to_f32(z[c]); }
+
+  // f(first column, N logits) by 16-byte loads from any element on, U of them on their way at a time; g(column, logit) for
+  // what is left at the end
+  template <int NT, int U, typename F, typename G>
+  __device__ __forceinline__ void vectors(F&& f, G&& g) const {
+    typedef typename std::conditional<N == 8, Vec8, Vec4>::type Bytes;
+    const int count = cols / N;
+    for (int i = threadIdx.x; i < count; i += NT * U) {
+      Vec16 v[U];
+      Bytes m[U];
 #pragma unroll
       for (int u = 0; u < U; u++) {
-        const int c = (i + u * NT < vectors ? i + u * NT : i) * N;
-        __builtin_memcpy(v[u], z + c, 16);
-        if (MASKED) __builtin_memcpy(m[u], mask + c, N);
+        const int c = (i + u * NT < count ? i + u * NT : i) * N;
+        v[u] = *(const GLOBAL Vec16*)(z + c);
+        if (MASKED) m[u] = *(const GLOBAL Bytes*)(mask + c);
       }
 #pragma unroll
       for (int u = 0; u < U; u++) {
-        const bool in = i + u * NT < vectors;
+        if (i + u * NT >= count) break;
+        T raw[N];
+        uint8_t open[N];
+        float x[N];
+        __builtin_memcpy(raw, &v[u], 16);
+        if (MASKED) __builtin_memcpy(open, &m[u], N);
 #pragma unroll
-        for (int n = 0; n < N; n++) {
-          f((i + u * NT) * N + n, in && !(MASKED && !m[u][n]) ? to_f32(v[u][n]) : -INFINITY);
-          if (ORDERED) __builtin_amdgcn_sched_barrier(0);
-        }
+        for (int n = 0; n < N; n++) x[n] = MASKED && !open[n] ? -INFINITY : to_f32(raw[n]);
+        f((i + u * NT) * N, x);
       }
     }
-    const int c = vectors * N + (int)threadIdx.x;
-    if (c < cols) f(c, !(MASKED && !mask[c]) ? to_f32(z[c]) : -INFINITY);
+    const int c = count * N + (int)threadIdx.x;
+    if (c < cols) g(c, (*this)(c));
+  }
+  // f(column, logit), one at a time: for rare passes, in little code
+  template <int NT, typename F>
+  __device__ __forceinline__ void each(F&& f) const {
+    for (int c = threadIdx.x; c < cols; c += NT) f(c, (*this)(c));
   }
 };
 
 __device__ __forceinline__ uint64_t place_of(float v, int c) { return (uint64_t)key_of(v) << 32 | (uint32_t)~c; }
 __device__ __forceinline__ float logit_of(uint64_t place) { return of_key((uint32_t)(place >> 32)); }
 __device__ __forceinline__ int64_t column_of(uint64_t place) { return (int64_t)(uint32_t)~(uint32_t)place; }
+
+// sorts G lanes' places, the larger first (bitonic, by exchanges between lanes); j: the lane's number among them
+template <int G, int K = 2, int M = 1>
+__device__ __forceinline__ uint64_t sort_lanes(uint64_t p, int j) {
+  if constexpr (K <= G) {
+    const uint64_t q = lane_xor<M>(p);
+    const bool larger = ((j & M) == 0) == ((j & K) == 0 || K == G);  // this lane keeps the larger one
+    p = (p > q) == larger ? p : q;
+    if constexpr (M > 1)
+      return sort_lanes<G, K, M / 2>(p, j);
+    else
+      return sort_lanes<G, 2 * K, K>(p, j);
+  } else {
+    return p;
+  }
+}
 
 // ---------------------------------------------------------------------------------------------- up to 64 categories
 // G lanes a row, one category each: sorted by exchanging places between lanes, then every setting is a prefix of the
@@ -166,23 +209,11 @@ __global__ __launch_bounds__(256) void sample_group(const T* logits, int64_t str
     const float v = in ? to_f32(logits[r * stride + j]) : -INFINITY;
     const bool nan = (__ballot(v != v) & group) != 0;
     uint64_t p = v == -INFINITY ? 0 : place_of(v, j);
-#pragma unroll
-    for (int k = 2; k <= G; k <<= 1)
-#pragma unroll
-      for (int m = k >> 1; m; m >>= 1) {
-        const uint64_t q = __shfl_xor((unsigned long long)p, m);
-        const bool larger = ((j & m) == 0) == ((j & k) == 0 || k == G);  // this lane keeps the larger one
-        p = (p > q) == larger ? p : q;
-      }
+    p = sort_lanes<G>(p, j);
     const int n = __popcll(__ballot(p != 0) & group);
     const float top = __shfl(logit_of(p), base);
     const uint64_t w = p && !nan ? weight_of(logit_of(p), top, o) : 0;
-    uint64_t sum = w;  // up to and with this lane's
-#pragma unroll
-    for (int m = 1; m < G; m <<= 1) {
-      const uint64_t q = __shfl_up((unsigned long long)sum, m, G);
-      if (j >= m) sum += q;
-    }
+    const uint64_t sum = sum_lanes<G>(w, j);  // up to and with this lane's
     int kept = o.top_k > 0 && o.top_k < n ? (int)o.top_k : n;
     auto upto = [&](int k) { return (uint64_t)__shfl((unsigned long long)sum, base + (k > 0 ? k - 1 : 0)); };
     uint64_t s = upto(kept);
@@ -209,11 +240,41 @@ struct List {
   int at;
 };
 
-// Sorts the first n places (the larger first) and sums their weights.  Bitonic: pairs that are at most 64 apart stay
-// within the 128 places of one wave, and need no barrier.  A place of 0 is none.
+// Sorts the first n places (the larger first) and sums their weights.  Up to 256, with as many threads as there are for
+// each, every place is compared with all (n^2 steps, but without a barrier between them: 200 places take 2 us, sorting them 9);
+// more are sorted by bitonic exchanges in LDS, where pairs that are at most 64 apart stay within the 128 places of one wave and
+// need no barrier.  A place of 0 is none.
 template <int NT, int LN>
-__device__ void sort_list(List<LN>& l, int n, float top, const Row& o) {
-  int m = 2;
+__device__ __forceinline__ void sort_list(List<LN>& l, int n, float top, const Row& o) {
+  constexpr int Q = NT > 256 ? NT / 256 : 1;  // threads for each place
+  if (n <= NT / Q) {
+    __syncthreads();
+    if ((int)threadIdx.x < n) {
+      const uint64_t p = l.place[threadIdx.x];
+      l.upto[threadIdx.x] = p ? weight_of(logit_of(p), top, o) : 0;
+    }
+    __syncthreads();
+    const int i = threadIdx.x / Q;
+    const uint64_t own = i < n ? l.place[i] : 0;
+    uint64_t sum = 0;
+    int before = 0;
+#pragma unroll 4
+    for (int k = threadIdx.x % Q; k < n; k += Q) {
+      const uint64_t p = l.place[k], w = l.upto[k];
+      sum += p >= own ? w : 0;
+      before += p > own || (p == own && k < i);  // (places of 0 are many)
+    }
+    sum = group_sum<Q>(sum);
+    before = group_sum<Q>(before);
+    __syncthreads();
+    if (i < n && threadIdx.x % Q == 0) {
+      l.place[before] = own;
+      l.upto[before] = sum;
+    }
+    __syncthreads();
+    return;
+  }
+  int m = 128;
   while (m < n) m <<= 1;
   for (int i = n + threadIdx.x; i < m; i += NT) l.place[i] = 0;
   __syncthreads();
@@ -238,22 +299,16 @@ __device__ void sort_list(List<LN>& l, int n, float top, const Row& o) {
   // each thread sums its share of the places, the shares are joined over lanes, then over waves
   const int each = (m + NT - 1) / NT, first = threadIdx.x * each;
   uint64_t own = 0;
-  for (int i = first; i < first + each && i < m; i++)
-    if (l.place[i]) own += weight_of(logit_of(l.place[i]), top, o);
-  uint64_t run = own;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const uint64_t x = __shfl_up((unsigned long long)run, d);
-    if ((threadIdx.x & 63) >= d) run += x;
+  for (int i = first; i < first + each && i < m; i++) {
+    own += l.place[i] ? weight_of(logit_of(l.place[i]), top, o) : 0;
+    l.upto[i] = own;
   }
+  const uint64_t run = sum_lanes<64>(own, threadIdx.x & 63);
   if ((threadIdx.x & 63) == 63) l.wave[threadIdx.x >> 6] = run;
   __syncthreads();
-  uint64_t sum = run - own;
-  for (int w = 0; w < (int)(threadIdx.x >> 6); w++) sum += l.wave[w];
-  for (int i = first; i < first + each && i < m; i++) {
-    if (l.place[i]) sum += weight_of(logit_of(l.place[i]), top, o);
-    l.upto[i] = sum;
-  }
+  uint64_t before = run - own;
+  for (int w = 0; w < (int)(threadIdx.x >> 6); w++) before += l.wave[w];
+  for (int i = first; i < first + each && i < m; i++) l.upto[i] += before;
   __syncthreads();
 }
 
@@ -298,18 +353,24 @@ __global__ __launch_bounds__(NT) void sample_list(const T* logits, int64_t strid
   __shared__ float fbuf[NT / 64];
   const int64_t r = blockIdx.x + (int64_t)gridDim.x * blockIdx.y;
   if (r < rows) {
-    const Source<T, MASKED> src{logits + r * stride, MASKED ? mask + r * mask_stride : nullptr, cols};
-    const Row o = block_settings(a, r);
+    const Source<T, MASKED> src{(const GLOBAL T*)(logits + r * stride), (const GLOBAL uint8_t*)(MASKED ? mask + r * mask_stride : nullptr), cols};
+    const Row o = uniform(row_settings(a, r));
     for (int c = threadIdx.x; c < cols; c += NT) l.place[c] = 0;
     __syncthreads();
     float top = -INFINITY;
     int wrong = o.nan, n = 0;
-    src.template each<NT, 1, false>([&](int c, float v) {
+    auto one = [&](int c, float v) {
       wrong |= v != v;
       top = fmaxf(top, v);
       n += v != -INFINITY;
       if (v != -INFINITY) l.place[c] = place_of(v, c);
-    });
+    };
+    src.template vectors<NT, 1>(
+        [&](int c, const float* v) {
+#pragma unroll
+          for (int i = 0; i < src.N; i++) one(c + i, v[i]);
+        },
+        one);
     top = block_max<NT>(top, fbuf);
     wrong = __syncthreads_or(wrong);
     n = block_sum<NT>(n, (int*)l.wave);
@@ -324,22 +385,198 @@ __global__ __launch_bounds__(NT) void sample_list(const T* logits, int64_t strid
 }
 
 // ---------------------------------------------------------------------------------------------- longer rows
-// One block a row.  A pass finds the largest logit, a second one counts and weighs the categories by how far below it
-// they lie (2048 steps of equal width); sums over steps then tell in which step a setting's border and the drawn
-// category lie, and only the categories of such a step, or of the few steps up to it, are listed and sorted.
-constexpr int NT = 1024, DIGIT = 11, BINS = 1 << DIGIT, LISTED = 2048;
+// One block a row, two passes over it as a rule.  The first counts or weighs the categories by steps of their logit, the
+// second lists and sorts those of the few steps in which a border and the drawn category lie.
+//
+// Steps are `scale` to a logit, counted down from HEAD at the largest logit of the row's first vectors (one for each
+// thread), so that no pass is needed to find the row's own largest; should one lie above step 0, the pass is made again.
+// With t = (first - v) scale + HEAD, step b = floor(t) and r = t - b, a category weighs exp(-r width) times what the top of its step
+// does, width = 1 / (scale T) <= 0.022 (32 steps to a power of two; more where the first vectors are closer together).  A
+// polynomial of degree 4 in r gives that to 5e-13 (four operations, 15 with the step's), and only the steps' sums are scaled
+// by a proper exp.  An equal logit weighs exactly as much: scale has 16 bits, which makes first * scale + HEAD, and with it t
+// of the first logit, exact.
+constexpr int BINS = 2048, HEAD = 512, DIGIT = 11;
 
-struct Find {
-  unsigned long long weight[BINS];
-  uint32_t count[BINS];
-  unsigned long long wave[NT / 64], ubuf[NT / 64];
-  unsigned long long place, before, upto;  // the category found; the sum before it and with it
-  float fbuf[2][NT / 64];
+struct Steps {
+  double first, scale, width;  // width: 1 / (scale T)
+  double base;                 // first * scale + HEAD
+  __device__ __forceinline__ double at(float v) const { return fma(-(double)v, scale, base); }
+  // never falls as v falls; -1 above the steps, the last step takes all that lies below
+  __device__ __forceinline__ static int of(double t) { return (int)floor(fmin(fmax(t, -1.0), (double)(BINS - 1))); }
+  __device__ __forceinline__ int operator()(float v) const { return of(at(v)); }
+  // all logits of steps b0 .. b1 (and a few others) lie within `half` of `mid`
+  __device__ __forceinline__ void around(int b0, int b1, float& mid, float& half) const {
+    const double d0 = (double)(HEAD - b0) / scale, d1 = (double)(HEAD - b1 - 1) / scale;
+    const double slack = 4e-7 * (fabs(first) + fabs(d0) + fabs(d1));
+    mid = (float)(first + 0.5 * (d0 + d1));
+    half = b0 > b1 ? -1.0f : b1 == BINS - 1 ? INFINITY : (float)(0.5 * (d0 - d1) + slack);
+  }
 };
+
+template <int NT>
+struct Long {
+  static constexpr int LISTED = NT;
+  List<LISTED> l;
+  unsigned long long weight[BINS + 1];
+  uint32_t count[BINS + 1];
+  unsigned long long wave[NT / 64], ubuf[NT / 64];
+  unsigned long long place, before, upto;  // find: the category found; the weight before it and with it
+  float fbuf[2][NT / 64];
+  unsigned long long tail;
+  int listed, step, seen, total;
+  // what the functions below, which are not inlined (each is called from several places), work on
+  const void* z;
+  const uint8_t* mask;
+  int cols;
+  float top;
+  Row o;
+  Steps steps;
+};
+template <int NT>
+__device__ __forceinline__ Long<NT>& shared() {
+  extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
+  return *(Long<NT>*)lds;
+}
+template <typename T, bool MASKED, int NT>
+__device__ __forceinline__ Source<T, MASKED> shared_source() {
+  const Long<NT>& g = shared<NT>();
+  return Source<T, MASKED>{uniform((const T*)g.z), MASKED ? uniform(g.mask) : nullptr, uniform(g.cols)};
+}
+// exclusive sums of `mine` over the block's threads, in order; `all` gets the sum of all
+template <int NT>
+__device__ __forceinline__ uint64_t block_before(uint64_t mine, unsigned long long* buf, uint64_t& all) {
+  const uint64_t run = sum_lanes<64>(mine, threadIdx.x & 63);
+  if ((threadIdx.x & 63) == 63) buf[threadIdx.x >> 6] = run;
+  __syncthreads();
+  uint64_t sum = 0, before = 0;
+#pragma unroll
+  for (int w = 0; w < NT / 64; w++) {
+    if (w == (int)(threadIdx.x >> 6)) before = sum;
+    sum += buf[w];
+  }
+  all = sum;
+  __syncthreads();
+  return before + run - mine;
+}
+
+// The first pass: counts and / or mantissas of every step.  Returns what only the row as a whole shows: its largest logit,
+// the number of its categories (COUNT), and as bits of `seen` a NaN (1) and a logit above the steps (2).  The last step's
+// count is what the others leave, its weight is g.tail.
+template <int NT, bool COUNT, bool WEIGH, typename S>
+__device__ __forceinline__ void weigh_steps(const S& src, const Steps& steps, double one, Long<NT>& g, float& top, int& categories, int& seen) {
+  constexpr double LOW = BINS - 1;
+  const bool far = (BINS - 1 - HEAD) * steps.width < 33.0;  // whether the last step can still weigh 2^-46 or more
+  // exp(-r width) = 1 + r (c1 + r (c2 + r (c3 + r c4))), exact at r = 0: its series with the term of r^5 put into the lower
+  // ones by r^4 = 2 r^3 - 5/4 r^2 + r/4 - 1/128, which Chebyshev's polynomial of degree 4 on 0 .. 1 gives to 1/128; 5e-13 in all.
+  // In units of 2^-s, and with 2^52 added, which leaves the whole number in the low bits
+  const double w = steps.width, e5 = -w * w * w * w * w / 120;
+  const double c1 = uniform(one * (-w - e5 / 128)), c2 = uniform(one * (w * w / 2 + e5 / 4));
+  const double c3 = uniform(one * (-w * w * w / 6 - e5 * 1.25)), c4 = uniform(one * (w * w * w * w / 24 + e5 * 2));
+  const double c0 = uniform(one + 4503599627370496.0);
+  // what lies in the steps; false for what may need a look: above them, NaN, and, where it can weigh, below them
+  auto fast = [&](float v) {
+    top = fmaxf(top, v);
+    if (COUNT) categories += v > -INFINITY;
+    const double t = steps.at(v);
+    const uint32_t upper = (uint32_t)(__double_as_longlong(t) >> 32);
+    const bool in = upper < 0x409FFC00u;  // 0 <= t < 2047, by its upper word: a sign or NaN makes that larger
+    if (in) {
+      const int b = (int)t;
+      if (COUNT) atomicAdd(&g.count[b], 1u);
+      if (WEIGH) {
+        const double r = __builtin_amdgcn_fract(t);
+        double e = fma(r, c4, c3);
+        e = fma(e, r, c2);
+        e = fma(e, r, c1);
+        e = fma(e, r, c0);
+        atomicAdd(&g.weight[b], (unsigned long long)__double_as_longlong(e) & 0xfffffffffffffull);
+      }
+    }
+    return in || (upper < 0x7ff00001u && !(WEIGH && far));
+  };
+  auto slow = [&](float v) {
+    const double t = steps.at(v);
+    if (!(t >= 0)) {
+      seen |= v != v ? 1 : 2;
+    } else if (WEIGH && t >= LOW && v > -INFINITY) {
+      const double e = exp_neg(fmax((LOW - t) * steps.width, -1000.0));
+      atomicAdd(&g.tail, (unsigned long long)__double_as_longlong(fma(e, one, 4503599627370496.0)) & 0xfffffffffffffull);
+    }
+  };
+  src.template vectors<NT, 2>(
+      [&](int c, const float* v) {
+        bool done = true;
+#pragma unroll
+        for (int i = 0; i < S::N; i++) {
+          done &= fast(v[i]);
+          __builtin_amdgcn_sched_barrier(0);  // one after the other: several at once spill registers
+        }
+        if (!done)
+#pragma unroll 1
+          for (int i = 0; i < S::N; i++) slow(src(c + i));
+      },
+      [&](int, float v) {
+        if (!fast(v)) slow(v);
+      });
+}
+
+// the step in which the running sum passes `number`
+template <int NT, typename V>
+__device__ __forceinline__ int step_of(Long<NT>& g, const V* sums, uint64_t number) {
+  for (int b = threadIdx.x; b < BINS; b += NT)
+    if (sums[b] <= number && number < sums[b + 1]) g.step = b;
+  __syncthreads();
+  const int b = g.step;
+  __syncthreads();
+  return b;
+}
+
+// Lists and sorts the categories of steps a0 .. a1 and b0 .. b1.  False, for all threads, where they are too many.
+template <typename T, bool MASKED, int NT>
+__device__ __noinline__ bool list_steps(int a0, int a1, int b0, int b1) {
+  Long<NT>& g = shared<NT>();
+  const Source<T, MASKED> src = shared_source<T, MASKED, NT>();
+  const Steps steps{uniform(g.steps.first), uniform(g.steps.scale), 0.0, uniform(g.steps.base)};
+  a0 = uniform(a0), a1 = uniform(a1), b0 = uniform(b0), b1 = uniform(b1);
+  if (threadIdx.x == 0) g.listed = 0;
+  __syncthreads();
+  // which step a logit lies in is computed only for those near the wanted ones
+  float am, ah, bm, bh;
+  steps.around(a0, a1, am, ah);
+  steps.around(b0, b1, bm, bh);
+  auto near = [&](float v) { return fabsf(v - am) <= ah || fabsf(v - bm) <= bh; };
+  auto take = [&](int c, float v) {
+    const int b = steps(v);
+    if (v == -INFINITY || !((b >= a0 && b <= a1) || (b >= b0 && b <= b1))) return;
+    const int i = atomicAdd(&g.listed, 1);
+    if (i < Long<NT>::LISTED) g.l.place[i] = place_of(v, c);
+  };
+  src.template vectors<NT, 4>(
+      [&](int c, const float* v) {
+        bool any = false;
+#pragma unroll
+        for (int i = 0; i < src.N; i++) any |= near(v[i]);
+        if (!any) return;
+        int hits = 0;
+#pragma unroll
+        for (int i = 0; i < src.N; i++) hits |= near(v[i]) ? 1 << i : 0;
+        for (; hits; hits &= hits - 1) {
+          const int i = c + __ffs(hits) - 1;
+          take(i, src(i));
+        }
+      },
+      take);
+  __syncthreads();
+  const int n = uniform(g.listed);
+  if (n > Long<NT>::LISTED) return false;
+  sort_list<NT>(g.l, n, uniform(g.top), uniform(g.o));
+  return true;
+}
 
 // adds a category to a bin; a wave whose categories all go to one bin adds them up first (one value in many places
 // would otherwise be 64 turns at the same address)
-__device__ __forceinline__ void add(Find& f, int b, uint64_t w) {
+template <int NT>
+__device__ __forceinline__ void add(Long<NT>& f, int b, uint64_t w) {
   const int b0 = __builtin_amdgcn_readfirstlane(b);
   if (__all(b == b0)) {
     const uint64_t active = __ballot(1);
@@ -356,13 +593,14 @@ __device__ __forceinline__ void add(Find& f, int b, uint64_t w) {
   atomicAdd(&f.weight[b], (unsigned long long)w);
 }
 
-// Of rows that the steps do not tell apart: the category at which a sum passes a number, digit by digit of its place.
-// Each pass over the row adds up its categories by the next 11 bits, among those that share the bits found so far.
-// The first category (in rank) at which the running sum of weights (or, by_count, of ones) is over `number`, which the
-// sum of all of them is.  f.place, f.before and f.upto (sums of weights) are set for every thread.
-template <typename S>
-__device__ __forceinline__ void find(bool by_count, const S& src, float top, const Row& o, uint64_t number, Find& f) {
-  const int low = 64 - __clz((unsigned)(src.cols > 1 ? src.cols - 1 : 1)) - 32;  // bits of an index
+// Of rows that the steps do not tell apart (more than a list of equal or nearly equal logits): the category at which a sum
+// passes a number, digit by digit of its place.  Each pass over the row adds up its categories by the next 11 bits,
+// among those that share the bits found so far.  Found is the first category (in rank) at which the running sum of
+// weights (or, by_count, of ones) is over `number`, which the sum of all of them is.  f.place, f.before and f.upto (sums of
+// weights) are set for every thread.
+template <int NT, typename S>
+__device__ __forceinline__ void find(bool by_count, const S& src, float top, const Row& o, uint64_t number, Long<NT>& f) {
+  const int low = 32 - __clz((unsigned)(src.cols - 1));  // bits of an index
   uint64_t place = 0, known = 0, before = 0, wbefore = 0;
   int at = 64;
   while (at > 0) {
@@ -378,49 +616,30 @@ __device__ __forceinline__ void find(bool by_count, const S& src, float top, con
       f.weight[i] = 0;
     }
     __syncthreads();
-    src.template each<NT, 2, true>([&](int c, float v) {
+    src.template each<NT>([&](int c, float v) {
       const uint64_t p = place_of(v, c);
       if (v > -INFINITY && (p & known) == place) add(f, (int)(p >> sh) & (bins - 1), weight_of(v, top, o));
     });
     __syncthreads();
     // thread i sums the i-th share of the bins from the top, then the bin is where the sum passes the number
-    const int each = (bins + NT - 1) / NT, first = bins - 1 - (int)threadIdx.x * each;
-    uint64_t own = 0, ownw = 0;
-    for (int i = 0; i < each && first - i >= 0; i++) {
-      own += by_count ? (uint64_t)f.count[first - i] : (uint64_t)f.weight[first - i];
-      ownw += f.weight[first - i];
+    const int each = (bins + NT - 1) / NT, last = bins - 1 - (int)threadIdx.x * each;
+    uint64_t own = 0, ownw = 0, all;
+    for (int i = 0; i < each && last - i >= 0; i++) {
+      own += by_count ? (uint64_t)f.count[last - i] : (uint64_t)f.weight[last - i];
+      ownw += f.weight[last - i];
     }
-    uint64_t run = own, runw = ownw;
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) {
-      const uint64_t x = __shfl_up((unsigned long long)run, m), y = __shfl_up((unsigned long long)runw, m);
-      if ((threadIdx.x & 63) >= m) {
-        run += x;
-        runw += y;
-      }
-    }
-    if ((threadIdx.x & 63) == 63) {
-      f.wave[threadIdx.x >> 6] = run;
-      f.ubuf[threadIdx.x >> 6] = runw;
-    }
-    __syncthreads();
-    uint64_t base = before, basew = wbefore;
-    for (int w = 0; w < (int)(threadIdx.x >> 6); w++) {
-      base += f.wave[w];
-      basew += f.ubuf[w];
-    }
-    uint64_t sum = base + run - own, sumw = basew + runw - ownw;
+    uint64_t sum = before + block_before<NT>(own, f.wave, all), sumw = wbefore + block_before<NT>(ownw, f.ubuf, all);
     if (sum <= number && number < sum + own) {  // one thread's
       for (int i = 0; i < each; i++) {
-        const uint64_t val = by_count ? (uint64_t)f.count[first - i] : (uint64_t)f.weight[first - i];
+        const uint64_t val = by_count ? (uint64_t)f.count[last - i] : (uint64_t)f.weight[last - i];
         if (number < sum + val) {
-          f.place = place | (uint64_t)(first - i) << sh;
+          f.place = place | (uint64_t)(last - i) << sh;
           f.before = sum;
           f.upto = sumw;
           break;
         }
         sum += val;
-        sumw += f.weight[first - i];
+        sumw += f.weight[last - i];
       }
     }
     __syncthreads();
@@ -440,212 +659,282 @@ __device__ __forceinline__ void find(bool by_count, const S& src, float top, con
   __syncthreads();
 }
 
-// the weight of the categories that min_p keeps: like every setting's, the leading part of the ranking
-template <typename S>
-__device__ __forceinline__ uint64_t weight_over(const S& src, float top, const Row& o, Find& f) {
-  uint64_t own = 0;
-  src.template each<NT, 2, true>([&](int, float v) {
+// the drawn category's place, with nothing but `find`
+template <typename T, bool MASKED, int NT>
+__device__ __noinline__ uint64_t draw_by_digits() {
+  Long<NT>& f = shared<NT>();
+  const Source<T, MASKED> src = shared_source<T, MASKED, NT>();
+  const float top = uniform(f.top);
+  const Row o = uniform(f.o);
+  uint64_t n = 0, all = 0, most = 0;  // categories, their weight, the weight of those that min_p keeps (a leading part, as every setting's)
+  src.template each<NT>([&](int, float v) {
     const uint64_t w = v > -INFINITY ? weight_of(v, top, o) : 0;
-    own += (double)w >= o.min_w ? w : 0;
+    n += v > -INFINITY;
+    all += w;
+    most += (double)w >= o.min_w ? w : 0;
   });
-  const uint64_t sum = block_sum<NT>((unsigned long long)own, f.ubuf);
+  n = block_sum<NT>((unsigned long long)n, f.ubuf);
   __syncthreads();
-  return sum;
-}
-
-// the drawn category's place, with nothing but `find`: n categories are not barred, their weight is `sum`, of which min_p
-// keeps at most `most`
-template <typename S>
-__device__ __forceinline__ uint64_t draw_by_digits(const S& src, float top, const Row& o, uint64_t n, uint64_t sum, uint64_t most, Find& f) {
+  all = block_sum<NT>((unsigned long long)all, f.ubuf);
+  __syncthreads();
+  most = block_sum<NT>((unsigned long long)most, f.ubuf);
+  __syncthreads();
+  uint64_t sum = all;
   for (int stage = 0;; stage++) {  // top_k's border, top_p's, the draw
-    if (stage == 0 && (o.greedy || o.top_k <= 0 || (uint64_t)o.top_k >= n)) continue;
-    if (stage == 1 && (o.greedy || o.top_p >= 1)) continue;
+    if (stage == 0 && (o.top_k <= 0 || (uint64_t)o.top_k >= n)) continue;
+    if (stage == 1 && o.top_p >= 1) continue;
     if (stage == 2 && most < sum) sum = most;
-    find(stage == 0 || o.greedy, src, top, o, o.greedy ? 0 : stage == 0 ? (uint64_t)o.top_k - 1 : stage == 1 ? border_of(o.top_p, sum) : target_of(o.u, sum), f);
+    find<NT>(stage == 0, src, top, o, stage == 0 ? (uint64_t)o.top_k - 1 : stage == 1 ? border_of(o.top_p, sum) : target_of(o.u, sum), f);
     if (stage == 2) return f.place;
     sum = f.upto;
     __syncthreads();
   }
 }
 
-// the step below the largest logit; a function that never falls as v does
-struct Steps {
-  float top, scale;
-  __device__ __forceinline__ int operator()(float v) const {
-    const float d = v == top ? 0.0f : (top - v) * scale;
-    return d < (float)(BINS - 1) ? (int)d : BINS - 1;
+// The drawn category's place from the steps' sums; 0 where a list is too short for it.
+template <typename T, bool MASKED, int NT>
+__device__ __forceinline__ uint64_t draw_by_steps(const Steps& steps, float top, const Row& o, bool counted, bool weighed) {
+  Long<NT>& g = shared<NT>();
+  const uint64_t n = counted ? g.count[BINS] : 0, all = weighed ? g.weight[BINS] : 0;
+  const bool cut = counted && (uint64_t)o.top_k < n;
+  uint64_t sum = all;
+  if (counted && !weighed) {  // top_k, and few: one list of all that it keeps (of all, where there are fewer)
+    const int to = cut ? step_of(g, g.count, (uint64_t)o.top_k - 1) : BINS - 1;
+    if (!list_steps<T, MASKED, NT>(0, to, 0, -1)) return 0;
+    return draw_from<NT>(g.l, g.listed, o);
   }
-};
-
-struct Long {
-  Find f;
-  List<LISTED> l;
-  int listed, step;
-  unsigned long long categories, weight;
-};
-
-// Lists and sorts the categories of steps `from` .. `to`.  False, for all threads, where they are too many.
-template <typename S>
-__device__ __forceinline__ bool list_steps(const S& src, const Steps& steps, int from, int to, const Row& o, Long& g) {
-  const uint32_t n = (to + 1 < BINS ? g.f.count[to + 1] : (uint32_t)g.categories) - g.f.count[from];
-  if (n > LISTED) return false;
-  __syncthreads();
-  if (threadIdx.x == 0) g.listed = 0;
-  __syncthreads();
-  src.template each<NT, 4, false>([&](int c, float v) {
-    const int b = steps(v);
-    if (b >= from && b <= to && v > -INFINITY) g.l.place[atomicAdd(&g.listed, 1)] = place_of(v, c);
-  });
-  __syncthreads();
-  sort_list<NT>(g.l, (int)n, steps.top, o);
-  return true;
+  if (cut) {
+    const int b = step_of(g, g.count, (uint64_t)o.top_k - 1);
+    if (!list_steps<T, MASKED, NT>(b, b, 0, -1)) return 0;
+    const int i = (int)(o.top_k - 1 - g.count[b]);
+    sum = g.weight[b] + g.l.upto[i < g.listed ? i : g.listed - 1];
+    __syncthreads();
+  }
+  // the steps of the border behind which nothing is kept: top_p's, or, where it comes first, min_p's (its logit is known
+  // but for rounding: three steps)
+  int b0 = BINS, b1 = -1;
+  if (o.top_p < 1) b0 = b1 = step_of(g, g.weight, border_of(o.top_p, sum));
+  if (o.min_w > 0) {
+    const double lowest = (double)top + (o.min_p < 1 ? log(fmax(o.min_p, 1e-300)) / o.inv_t : 0.0);
+    const int m = Steps::of((steps.first - lowest) * steps.scale + HEAD);
+    const int m0 = m > 1 ? m - 1 : 0, m1 = m + 1 < BINS ? m + 1 : BINS - 1;
+    if (b1 < 0 || m1 < b0) {
+      b0 = m0;
+      b1 = m1;
+    } else if (m0 <= b1) {
+      b0 = m0 < b0 ? m0 : b0;
+      b1 = m1 > b1 ? m1 : b1;
+    }
+  }
+  const bool border = b1 >= 0;
+  // the draw's step is known but for how much of the border's steps is kept
+  int t0 = step_of(g, g.weight, target_of(o.u, border && g.weight[b0] ? (uint64_t)g.weight[b0] : border ? 1 : sum));
+  int t1 = border ? step_of(g, g.weight, target_of(o.u, (uint64_t)g.weight[b1 + 1] < sum ? (uint64_t)g.weight[b1 + 1] : sum)) : t0;
+  for (int turn = 0; turn < 2; turn++) {
+    // first both in one list, then, should they be too many, the border alone and the one step of the draw
+    if (turn && !border) return 0;
+    const bool together = turn == 0;
+    const bool joined = together && border && b0 <= t1 + 1;  // one stretch of steps
+    if (together ? list_steps<T, MASKED, NT>(t0, border && t1 > b1 ? b1 : t1, b0, b1) : list_steps<T, MASKED, NT>(b0, b1, 0, -1)) {
+      int split = 0;  // where the border's steps begin
+      uint64_t base = g.weight[border ? (joined ? (t0 < b0 ? t0 : b0) : b0) : t0];
+      const uint64_t tbase = joined ? base : g.weight[t0];
+      if (together && border && !joined) {
+        if (threadIdx.x == 0) g.step = 0;
+        __syncthreads();
+        for (int i = threadIdx.x; i < g.listed; i += NT)
+          if (steps(logit_of(g.l.place[i])) <= t1) atomicMax(&g.step, i + 1);
+        __syncthreads();
+        split = g.step;
+        __syncthreads();
+      }
+      const uint64_t off = split ? g.l.upto[split - 1] : 0;  // of the list's sum, what belongs to the draw's steps
+      if (border) {
+        int end = g.listed;  // what is kept of the list
+        if (o.top_p < 1) {
+          const uint64_t number = border_of(o.top_p, sum);
+          end = number < base ? split : first_over<NT>(g.l, end, number - base + off) + 1;
+        }
+        if (o.min_w > 0) {
+          if (threadIdx.x == 0) g.step = 0;
+          __syncthreads();
+          for (int i = threadIdx.x; i < end; i += NT)
+            if ((double)(g.l.upto[i] - (i ? g.l.upto[i - 1] : 0)) >= o.min_w) atomicMax(&g.step, i + 1);
+          __syncthreads();
+          end = g.step;
+          __syncthreads();
+        }
+        const uint64_t kept = base + (end > split ? g.l.upto[end - 1] - off : 0);
+        sum = kept < sum ? kept : sum;
+      }
+      const uint64_t number = target_of(o.u, sum);
+      if (together) return g.l.place[first_over<NT>(g.l, border && !joined ? split : g.listed, number < tbase ? 0 : number - tbase)];
+      const int b = step_of(g, g.weight, number);
+      if (!list_steps<T, MASKED, NT>(b, b, 0, -1)) return 0;
+      return g.l.place[first_over<NT>(g.l, g.listed, number - g.weight[b])];
+    }
+  }
+  return 0;
 }
 
-// the step in which the running count (or weight) passes `number`
-__device__ __forceinline__ int step_of(bool by_count, Long& g, uint64_t number) {
-  for (int b = threadIdx.x; b < BINS; b += NT) {
-    const uint64_t from = by_count ? (uint64_t)g.f.count[b] : (uint64_t)g.f.weight[b];
-    const uint64_t to = b + 1 == BINS ? (by_count ? g.categories : g.weight) : by_count ? (uint64_t)g.f.count[b + 1] : (uint64_t)g.f.weight[b + 1];
-    if (from <= number && number < to) g.step = b;
-  }
-  __syncthreads();
-  const int b = g.step;
-  __syncthreads();
-  return b;
-}
-
-template <typename T, bool MASKED>
-__global__ __launch_bounds__(NT) void sample_long(const T* logits, int64_t stride, const uint8_t* mask, int64_t mask_stride, Settings a, int64_t* out,
+template <typename T, bool MASKED, int NT>
+__global__ __launch_bounds__(NT, 4) void sample_long(const T* logits, int64_t stride, const uint8_t* mask, int64_t mask_stride, Settings a, int64_t* out,
                                                   int64_t rows, int cols) {
-  __shared__ Long g;
+  Long<NT>& g = shared<NT>();
   const int64_t r = blockIdx.x + (int64_t)gridDim.x * blockIdx.y;
-  if (r < rows) {
-    const Source<T, MASKED> src{logits + r * stride, MASKED ? mask + r * mask_stride : nullptr, cols};
-    const Row o = block_settings(a, r);
-    float top = -INFINITY, least = INFINITY;
-    int wrong = o.nan;
-    src.template each<NT, 4, false>([&](int, float v) {
+  if (r >= rows) return;
+  const Source<T, MASKED> src{(const GLOBAL T*)(logits + r * stride), (const GLOBAL uint8_t*)(MASKED ? mask + r * mask_stride : nullptr), cols};
+  const Row o = uniform(row_settings(a, r));
+  float top = -INFINITY;
+  int wrong = o.nan;
+  uint64_t found = 0;
+  if (o.greedy || wrong) {
+    unsigned long long best = 0;
+    auto larger = [&](int c, float v) {
       wrong |= v != v;
-      top = fmaxf(top, v);
-      least = fminf(least, v > -INFINITY ? v : INFINITY);
-    });
-    for (int b = threadIdx.x; b < BINS; b += NT) {
-      g.f.count[b] = 0;
-      g.f.weight[b] = 0;
-    }
-    top = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(block_max<NT>(top, g.f.fbuf[0]))));
-    least = -block_max<NT>(-least, g.f.fbuf[1]);
-    wrong = __syncthreads_or(wrong);
-    uint64_t found = 0;
-    if (!wrong && top > -INFINITY) {
-      // steps of 1/64 of the temperature reach down to weights of e^-32; narrower where the whole row is closer
-      const float wanted = fmaxf(64.0f * (float)fabs(o.inv_t), (float)BINS / (top - least));
-      const Steps steps{top, wanted < 1e30f ? wanted : 1e30f};
-      src.template each<NT, 2, true>([&](int, float v) {
-        if (v > -INFINITY) add(g.f, steps(v), weight_of(v, top, o));
-      });
-      __syncthreads();
-      {  // counts and weights to sums of the steps before; two steps a thread
-        const int b = threadIdx.x * 2;
-        const uint32_t c0 = g.f.count[b], c1 = g.f.count[b + 1];
-        const uint64_t w0 = g.f.weight[b], w1 = g.f.weight[b + 1];
-        uint64_t c = c0 + c1, w = w0 + w1;
+      const unsigned long long p = v > -INFINITY ? place_of(v, c) : 0;
+      best = p > best ? p : best;
+    };
+    src.template vectors<NT, 2>(
+        [&](int c, const float* v) {
 #pragma unroll
-        for (int m = 1; m < 64; m <<= 1) {
-          const uint64_t x = __shfl_up((unsigned long long)c, m), y = __shfl_up((unsigned long long)w, m);
-          if ((threadIdx.x & 63) >= m) {
-            c += x;
-            w += y;
-          }
-        }
-        if ((threadIdx.x & 63) == 63) {
-          g.f.wave[threadIdx.x >> 6] = c;
-          g.f.ubuf[threadIdx.x >> 6] = w;
-        }
-        __syncthreads();
-        for (int v = 0; v < (int)(threadIdx.x >> 6); v++) {
-          c += g.f.wave[v];
-          w += g.f.ubuf[v];
-        }
-        g.f.count[b] = (uint32_t)c - c0 - c1;
-        g.f.count[b + 1] = (uint32_t)c - c1;
-        g.f.weight[b] = w - w0 - w1;
-        g.f.weight[b + 1] = w - w1;
-        if (threadIdx.x == NT - 1) {
-          g.categories = c;
-          g.weight = w;
-        }
-        __syncthreads();
-      }
-      const uint64_t n = g.categories, all = g.weight;
-      const bool cut = o.top_k > 0 && (uint64_t)o.top_k < n;
-      uint64_t sum = all, most = all;
-      bool ok = false;
-      // First, one list of every step that can hold a kept category: few categories, as a rule.  Else a list for each
-      // border, of its own step: top_k's, top_p's, the draw's.
-      for (int stage = 0; stage < 4; stage++) {
-        int from = 0, to = BINS - 1;
-        uint64_t number = 0;
-        if (stage == 0) {
-          if (o.greedy)
-            to = 0;
-          else if (cut)
-            to = step_of(true, g, (uint64_t)o.top_k - 1);
-          else if (o.top_p < 1)
-            to = step_of(false, g, border_of(o.top_p, all));
-          if (o.min_p > 1e-9 && !o.greedy && !(cut && o.top_p < 1)) {
-            // min_p keeps logits over top + T ln(min_p); a step more than that, and some float32 roundings, are let in.
-            // (With both others, top_p's share is of all that top_k keeps: none of it can be left out.)
-            const double reach = log(fmin(o.min_p, 1.0)) / o.inv_t, least_kept = (double)top + reach * 1.000001 - 1e-6 * fabs((double)top);
-            const int last = steps((float)least_kept) + 1;
-            to = last < to ? last : to;
-          }
-        } else if (stage == 1) {
-          if (!cut) continue;
-          from = to = step_of(true, g, (uint64_t)o.top_k - 1);
-        } else {
-          if (stage == 2 && o.top_p >= 1) continue;
-          if (stage == 3 && o.min_w > 0) {
-            most = weight_over(src, top, o, g.f);
-            sum = most < sum ? most : sum;
-          }
-          number = stage == 2 ? border_of(o.top_p, sum) : target_of(o.u, sum);
-          from = to = step_of(false, g, number);
-        }
-        ok = list_steps(src, steps, from, to, o, g);
-        if (!ok) {
-          if (stage == 0 && !o.greedy) continue;
-          break;
-        }
-        const int listed = g.listed;
-        if (stage == 0) {
-          Row rest = o;
-          int m = listed;
-          if (!cut && o.top_p < 1 && !o.greedy) {  // top_p's share is of the whole row, which the list is not
-            m = first_over<NT>(g.l, listed, border_of(o.top_p, all)) + 1;
-            rest.top_p = 1;
-          }
-          found = draw_from<NT>(g.l, m, rest);
-          break;
-        }
-        if (stage == 1) {
-          sum = g.f.weight[from] + g.l.upto[o.top_k - 1 - g.f.count[from]];
-        } else {
-          const int at = first_over<NT>(g.l, listed, number - g.f.weight[from]);
-          if (stage == 2)
-            sum = g.f.weight[from] + g.l.upto[at];
-          else
-            found = g.l.place[at];
-        }
-      }
-      if (!ok) {
-        __syncthreads();
-        if (o.min_w > 0 && !o.greedy) most = weight_over(src, top, o, g.f);
-        found = draw_by_digits(src, top, o, n, all, most, g.f);
-      }
-    }
-    if (threadIdx.x == 0) out[r] = found ? column_of(found) : -1;
+          for (int i = 0; i < src.N; i++) larger(c + i, v[i]);
+        },
+        larger);
+    best = sort_lanes<64>(best, threadIdx.x & 63);  // the largest to lane 0
+    if ((threadIdx.x & 63) == 0) g.wave[threadIdx.x >> 6] = best;
+    wrong = __syncthreads_or(wrong);
+    for (int w = 0; w < NT / 64; w++) best = g.wave[w] > best ? g.wave[w] : best;
+    if (threadIdx.x == 0) out[r] = wrong || !best ? -1 : column_of(best);
+    return;
   }
+  // the first vectors: where the steps start and how narrow they can be
+  const Source<T, MASKED> start{src.z, src.mask, cols < NT * (16 / (int)sizeof(T)) ? cols : NT * (16 / (int)sizeof(T))};
+  float first = -INFINITY, least = INFINITY;
+  auto look = [&](int, float v) {
+    first = fmaxf(first, v);
+    least = fminf(least, v > -INFINITY ? v : INFINITY);
+  };
+  start.template vectors<NT, 1>(
+      [&](int c, const float* v) {
+#pragma unroll
+        for (int i = 0; i < src.N; i++) look(c + i, v[i]);
+      },
+      look);
+  for (int b = threadIdx.x; b < BINS; b += NT) {
+    g.count[b] = 0;
+    g.weight[b] = 0;
+  }
+  first = group_max<64>(first);
+  least = -group_max<64>(-least);
+  if ((threadIdx.x & 63) == 0) {
+    g.fbuf[0][threadIdx.x >> 6] = first;
+    g.fbuf[1][threadIdx.x >> 6] = least;
+  }
+  __syncthreads();
+  for (int w = 0; w < NT / 64; w++) {
+    first = fmaxf(first, g.fbuf[0][w]);
+    least = fminf(least, g.fbuf[1][w]);
+  }
+  const bool counted = o.top_k > 0 && o.top_k < cols, weighed = !counted || o.top_k > NT / 2;
+  for (int turn = 0; turn < 2; turn++) {
+    // a power of two of the weight in 32 steps; narrower where the first vectors all lie within 1024 of them
+    // T counts as 2^-35 |first| at least: the next float32 below would still weigh e^-2048, and first * scale stays below 2^41
+    const double most = 34359738368.0 / fabs((double)first), inv_t = fmin(o.inv_t, most);
+    const double wanted = fmin(fmin(fmax(32.0 * 1.4426950408889634 * inv_t, 1024.0 / ((double)first - (double)least)), 64.0 * most), 1e300);
+    Steps steps;
+    steps.first = uniform(first);
+    steps.scale = uniform(__longlong_as_double(__double_as_longlong(wanted) >> 37 << 37));
+    steps.width = uniform(inv_t / steps.scale);
+    steps.base = uniform(steps.first * steps.scale + HEAD);
+    if (turn)
+      for (int b = threadIdx.x; b < BINS; b += NT) {
+        g.count[b] = 0;
+        g.weight[b] = 0;
+      }
+    if (threadIdx.x == 0) g.tail = g.total = 0;
+    __syncthreads();
+    int seen = 0;
+    top = -INFINITY;
+    int categories = 0;
+    if (!(first > -INFINITY && first < INFINITY)) {  // nothing to start from, or nothing but infinity counts
+      seen = 2;
+      src.template each<NT>([&](int, float v) {
+        seen |= v != v;
+        top = fmaxf(top, v);
+      });
+    } else if (!weighed) {
+      weigh_steps<NT, true, false>(src, steps, o.one, g, top, categories, seen);
+    } else if (!counted) {
+      weigh_steps<NT, false, true>(src, steps, o.one, g, top, categories, seen);
+    } else {
+      weigh_steps<NT, true, true>(src, steps, o.one, g, top, categories, seen);
+    }
+    if (threadIdx.x == 0) {
+      g.z = (const void*)src.z;
+      g.mask = (const uint8_t*)src.mask;
+      g.cols = cols;
+      g.o = o;
+      g.steps = steps;
+      g.seen = 0;
+    }
+    __syncthreads();
+    if (seen) atomicOr(&g.seen, seen);
+    if (counted) {
+      categories = group_sum<64>(categories);
+      if ((threadIdx.x & 63) == 0) atomicAdd(&g.total, categories);
+    }
+    top = block_max<NT>(top, g.fbuf[0]);  // (a barrier)
+    if (threadIdx.x == 0) g.top = top;
+    seen = uniform(g.seen);
+    if ((seen & 1) || top == -INFINITY) break;
+    if (seen) {
+      // again from the row's largest logit; rows of infinities are left to the digits
+      if (turn == 0 && top < INFINITY) {
+        least = fminf(least, top);
+        first = top;
+        __syncthreads();
+        continue;
+      }
+      __syncthreads();
+      found = draw_by_digits<T, MASKED, NT>();
+      break;
+    }
+    // the steps' mantissas to weights; counts and weights to sums of the steps before
+    constexpr int EACH = BINS / NT;
+    const int b0 = threadIdx.x * EACH;
+    uint64_t all;
+    if (weighed) {
+      const double shift = ((double)top - steps.first) * inv_t;
+      uint64_t sum = 0;
+      for (int i = 0; i < EACH; i++) {
+        const uint64_t m = b0 + i < BINS - 1 ? g.weight[b0 + i] : g.tail;
+        const uint64_t w = m ? (uint64_t)rint((double)m * exp_neg(fmax((double)(HEAD - b0 - i) * steps.width - shift, -1000.0))) : 0;
+        g.weight[b0 + i] = sum;
+        sum += w;
+      }
+      sum = block_before<NT>(sum, g.wave, all);
+      for (int i = 0; i < EACH; i++) g.weight[b0 + i] += sum;
+      if (threadIdx.x == 0) g.weight[BINS] = all;
+    }
+    if (counted) {
+      uint32_t sum = 0;
+      for (int i = 0; i < EACH; i++) {
+        const uint32_t c = g.count[b0 + i];
+        g.count[b0 + i] = sum;
+        sum += c;
+      }
+      sum = (uint32_t)block_before<NT>(sum, g.ubuf, all);
+      for (int i = 0; i < EACH; i++) g.count[b0 + i] += sum;
+      if (threadIdx.x == 0) g.count[BINS] = (uint32_t)g.total;
+    }
+    __syncthreads();
+    found = draw_by_steps<T, MASKED, NT>(steps, top, o, counted, weighed);
+    __syncthreads();
+    if (!found) found = draw_by_digits<T, MASKED, NT>();
+    break;
+  }
+  if (threadIdx.x == 0) out[r] = found ? column_of(found) : -1;
 }
 
 int shift_of(int64_t cols) {  // the sum of cols weights of at most 2^s stays below 2^63
@@ -687,8 +976,10 @@ void launch(const fm_sample_args& a) {
     sample_list<T, MASKED, 256, 1024><<<each, 256, 0, st>>>(ARGS);
   else if (cols <= 2048)
     sample_list<T, MASKED, 512, 2048><<<each, 512, 0, st>>>(ARGS);
+  else if (a.rows >= 1024 || cols <= 4096)
+    sample_long<T, MASKED, 256><<<each, 256, sizeof(Long<256>), st>>>(ARGS);
   else
-    sample_long<T, MASKED><<<each, NT, 0, st>>>(ARGS);
+    sample_long<T, MASKED, 1024><<<each, 1024, sizeof(Long<1024>), st>>>(ARGS);
 #undef ARGS
 }
 }  // namespace
