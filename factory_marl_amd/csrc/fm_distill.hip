@@ -10,6 +10,8 @@
 namespace fm {
 namespace {
 constexpr int NT = 256;
+constexpr int SHORT = 2048;   // columns of a row that a group of lanes takes
+constexpr int SPLIT = 32768;  // columns of a row that a block takes, backward
 
 struct Teacher {
   const void* index;
@@ -148,8 +150,9 @@ __device__ __forceinline__ Softmax softmax_of(const T* zr, int j, const Teacher&
   return q;
 }
 
-__device__ __forceinline__ double term_of(float p, float teacher, float top, double log_total, float z, float m, double log_s, const Teacher& t) {
-  return (double)p * ((((double)teacher - top) - ((double)z - m)) * t.inv_t - log_total + log_s);
+// one entry's part of the loss; log_ratio: log of the student's sum of exp over the teacher's
+__device__ __forceinline__ double term_of(float p, float teacher, float top, float z, float m, double log_ratio, const Teacher& t) {
+  return (double)p * ((((double)teacher - top) - ((double)z - m)) * t.inv_t + log_ratio);
 }
 
 template <typename T, int G, bool WIDE>
@@ -162,7 +165,7 @@ __global__ __launch_bounds__(NT) void distill_fwd_group(const T* z, int64_t stri
     const Entry e = entry_of<G>(t, r, j, group);
     const Softmax q = softmax_of<T, G, WIDE>(zr, j, t);
     double sum = 0;
-    if (e.p > 0) sum = term_of(e.p, e.logit, e.top, log((double)e.total), to_f32(zr[e.at]), q.m, log((double)q.s), t);
+    if (e.p > 0) sum = term_of(e.p, e.logit, e.top, to_f32(zr[e.at]), q.m, log((double)q.s / e.total), t);
     sum = group_sum<G>(sum);
     if (j || row >= rows) continue;
     loss[row] = e.mass != e.mass ? e.mass : e.mass == 0 ? 0.0f : (float)(t.t2 * sum);
@@ -173,49 +176,60 @@ __global__ __launch_bounds__(NT) void distill_fwd_group(const T* z, int64_t stri
   }
 }
 
+// Everything first as if nothing were listed, then the listed columns again, each by the lanes whose entries list it: by p
+// of the one entry, or, where a column is listed twice (a bit of it is set twice), by all entries' sum, the same for each of them.
 template <typename T, int G, bool WIDE>
 __global__ __launch_bounds__(NT) void distill_bwd_group(const T* z, int64_t stride, Teacher t, const float* stats, const float* grad, int64_t grad_stride,
                                                         T* dz, int64_t rows) {
+  constexpr int N = 16 / (int)sizeof(T), WORDS = WIDE ? SHORT / 32 : G / 32 + (G < 32);
+  __shared__ uint32_t bits[NT / G][WORDS];
   const int lane = threadIdx.x & 63, j = lane & (G - 1), base = lane - j;
   const uint64_t group = (G == 64 ? ~0ull : (1ull << G) - 1) << base;
+  uint32_t* seen = bits[threadIdx.x / G];
   for (int64_t first = (int64_t)blockIdx.x * (NT / G); first < rows; first += (int64_t)gridDim.x * (NT / G)) {
     const int64_t row = first + threadIdx.x / G, r = row < rows ? row : rows - 1;
     const T* zr = z + r * stride;
     T* dr = dz + r * (int64_t)t.cols;
     const Entry e = entry_of<G>(t, r, j, group);
+    for (int i = j; i < WORDS; i += G) seen[i] = 0;
+    wave_sync();
+    bool twice = false;
+    if (e.at >= 0) twice = atomicOr(&seen[e.at >> 5], 1u << (e.at & 31)) >> (e.at & 31) & 1;
     const float m = stats[2 * r], inv = 1.0f / stats[2 * r + 1], scale = e.mass == 0 ? 0.0f : e.mass * grad[r * grad_stride] * t.temperature;
     auto part = [&](float v, float listed) { return e.mass == 0 ? 0.0f : scale * (exp2_neg((v - m) * t.c) * inv - listed); };
-    // what the row's entries list at column c of each lane's own
-    auto listed_at = [&](int c) {
-      float listed = 0;
-      for (int i = 0; i < t.k; i++) {
-        const int at = __shfl(e.at, base + i);
-        const float p = __shfl(e.p, base + i);
-        listed += at == c ? p : 0.0f;
-      }
-      return listed;
-    };
-    if (!WIDE) {
-      const float listed = listed_at(j);
-      if (j < t.cols && row < rows) dr[j] = from_f32<T>(part(to_f32(zr[j]), listed));
-      continue;
-    }
-    if (row < rows) {  // the same for the whole wave
-      constexpr int N = 16 / (int)sizeof(T);
-      each<2>(
-          zr, 0, t.cols, j, 64,
-          [&](int c, const float* v) {
-            T o[N];
+    if (row < rows) {
+      if (WIDE) {
+        each<2>(
+            zr, 0, t.cols, j, 64,
+            [&](int c, const float* v) {
+              T o[N];
 #pragma unroll
-            for (int n = 0; n < N; n++) o[n] = from_f32<T>(part(v[n], 0.0f));
-            __builtin_memcpy(dr + c, o, 16);
-          },
-          [&](int c, float v) { dr[c] = from_f32<T>(part(v, 0.0f)); });
-      const float listed = listed_at(e.at);
-      wave_sync();
-      // the listed columns again: whoever lists the same one writes the same value
-      if (e.at >= 0 && e.mass == 1) dr[e.at] = from_f32<T>(part(to_f32(zr[e.at]), listed));
+              for (int n = 0; n < N; n++) o[n] = from_f32<T>(part(v[n], 0.0f));
+              __builtin_memcpy(dr + c, o, 16);
+            },
+            [&](int c, float v) { dr[c] = from_f32<T>(part(v, 0.0f)); });
+      } else if (j < t.cols) {
+        dr[j] = from_f32<T>(part(to_f32(zr[j]), 0.0f));
+      }
     }
+    float listed = e.p;
+    if (__ballot(twice)) {  // in any of the wave's rows
+      listed = 0;
+      for (int i = 0; i < t.k; i++) {
+        int at;
+        float p;
+        if (G == 64) {
+          at = __builtin_amdgcn_readlane(e.at, i);
+          p = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(e.p), i));
+        } else {
+          at = __shfl(e.at, base + i);
+          p = __shfl(e.p, base + i);
+        }
+        listed += at == e.at ? p : 0.0f;
+      }
+    }
+    wave_sync();
+    if (e.at >= 0 && e.mass == 1 && row < rows) dr[e.at] = from_f32<T>(part(to_f32(zr[e.at]), listed));
   }
 }
 
@@ -243,10 +257,10 @@ __device__ __forceinline__ void write_loss(const T* zr, const Teacher& t, int64_
                                            double* dbuf) {
   float top, total;
   const float mass = load_teacher(t, r, at, p, buf, top, total);
-  const double log_s = log((double)q.s), log_total = log((double)total);
+  const double log_ratio = log((double)q.s / total);
   double sum = 0;
   for (int i = threadIdx.x; i < t.k; i += NT)
-    if (p[i] > 0) sum += term_of(p[i], logit_at(t, r, i), top, log_total, to_f32(zr[at[i]]), q.m, log_s, t);
+    if (p[i] > 0) sum += term_of(p[i], logit_at(t, r, i), top, to_f32(zr[at[i]]), q.m, log_ratio, t);
   sum = block_sum<NT>(sum, dbuf);
   if (threadIdx.x) return;
   loss[r] = mass != mass ? mass : mass == 0 ? 0.0f : (float)(t.t2 * sum);
@@ -298,20 +312,30 @@ __global__ __launch_bounds__(NT) void distill_fwd_join(const T* z, int64_t strid
 }
 
 // dlogits of a split of a row a block: everything first as if nothing were listed, then the listed columns of the split
-// again, each with all of the entries that list it (whoever lists the same one writes the same value).
+// again, as above (whoever lists the same one writes the same value).
 template <typename T>
 __global__ __launch_bounds__(NT) void distill_bwd(const T* z, int64_t stride, Teacher t, const float* stats, const float* grad, int64_t grad_stride, T* dz,
                                                   int64_t rows, int splits) {
   __shared__ int at[FM_DISTILL_MAX_K];
   __shared__ float p[FM_DISTILL_MAX_K], buf[3 * (NT / 64)];
+  __shared__ uint32_t seen[SPLIT / 32 + 1], dup[SPLIT / 32 + 1];  // columns of the split that are listed, and listed twice
   const int64_t b = blockIdx.x + (int64_t)gridDim.x * blockIdx.y, r = b / splits;
   if (r >= rows) return;
   const T* zr = z + r * stride;
   T* dr = dz + r * (int64_t)t.cols;
   int from, to;
   split_of<T>(t.cols, (int)(b - r * splits), splits, from, to);
+  for (int i = threadIdx.x; i < SPLIT / 32 + 1; i += NT) seen[i] = dup[i] = 0;
   float top, total;
   const float mass = load_teacher(t, r, at, p, buf, top, total);
+  int twice = 0;  // whether a column of the split is listed twice
+  for (int i = threadIdx.x; i < t.k; i += NT) {
+    const int c = at[i] - from;
+    if (at[i] >= from && at[i] < to && (atomicOr(&seen[c >> 5], 1u << (c & 31)) >> (c & 31) & 1)) {
+      twice = 1;
+      atomicOr(&dup[c >> 5], 1u << (c & 31));
+    }
+  }
   const float m = stats[2 * r], inv = 1.0f / stats[2 * r + 1], scale = mass == 0 ? 0.0f : mass * grad[r * grad_stride] * t.temperature;
   auto part = [&](float v, float listed) { return mass == 0 ? 0.0f : scale * (exp2_neg((v - m) * t.c) * inv - listed); };
   constexpr int N = 16 / (int)sizeof(T);
@@ -325,13 +349,23 @@ __global__ __launch_bounds__(NT) void distill_bwd(const T* z, int64_t stride, Te
       },
       [&](int c, float v) { dr[c] = from_f32<T>(part(v, 0.0f)); });
   if (mass != 1) return;
-  __syncthreads();
-  for (int i = threadIdx.x; i < t.k; i += NT) {
-    const int c = at[i];
-    if (c < from || c >= to) continue;
-    float listed = 0;
-    for (int n = 0; n < t.k; n++) listed += at[n] == c ? p[n] : 0.0f;
-    dr[c] = from_f32<T>(part(to_f32(zr[c]), listed));
+  twice = __syncthreads_or(twice);
+  for (int first = threadIdx.x & ~63; first < t.k; first += NT) {  // a wave at a time: 64 entries
+    const int i = first + (threadIdx.x & 63), c = i < t.k ? at[i] : -1;
+    const bool mine = c >= from && c < to;
+    float listed = mine ? p[i] : 0.0f;
+    if (twice) {
+      // the entries whose column is listed twice, one after the other: all of the wave's lanes look for it
+      uint64_t left = __ballot(mine && (dup[(c - from) >> 5] >> ((c - from) & 31) & 1));
+      for (; left; left &= left - 1) {
+        const int lane = __ffsll((unsigned long long)left) - 1, column = __builtin_amdgcn_readlane(c, lane);
+        float sum = 0;
+        for (int n = threadIdx.x & 63; n < t.k; n += 64) sum += at[n] == column ? p[n] : 0.0f;
+        sum = group_sum<64>(sum);
+        if ((threadIdx.x & 63) == lane) listed = sum;
+      }
+    }
+    if (mine) dr[c] = from_f32<T>(part(to_f32(zr[c]), listed));
   }
 }
 
@@ -352,7 +386,7 @@ int splits_of(int64_t rows, int64_t cols) {
 // f(lanes, wide) for rows and lists that a group of lanes holds; false for longer ones
 template <typename F>
 bool with_group(int64_t cols, int64_t k, F&& f) {
-  if (k > 64 || cols > 2048) return false;
+  if (k > 64 || cols > SHORT) return false;
 #define GROUP(g, w) f(std::integral_constant<int, g>(), std::integral_constant<bool, w>())
   const int64_t n = cols > k ? cols : k;
   if (n <= 2)
@@ -406,8 +440,8 @@ void backward(const fm_distill_args& a) {
             <<<(int)(n < (1 << 20) ? n : 1 << 20), NT, 0, st>>>(z, a.stride, t, a.stats, a.grad, a.grad_stride, (T*)a.dlogits, a.rows);
       }))
     return;
-  // a block for every 32768 columns (the list is read again for each), for fewer where that leaves CUs without work
-  int64_t splits = (a.cols + 32767) / 32768;
+  // a block for every SPLIT columns (the list is read again for each), for fewer where that leaves CUs without work
+  int64_t splits = (a.cols + SPLIT - 1) / SPLIT;
   if (a.rows * splits < 1024) splits = splits_of(a.rows, a.cols) > splits ? splits_of(a.rows, a.cols) : splits;
   distill_bwd<T><<<grid_of(a.rows * splits), NT, 0, st>>>(z, a.stride, t, a.stats, a.grad, a.grad_stride, (T*)a.dlogits, a.rows, (int)splits);
 }

@@ -10,27 +10,83 @@ namespace fm {
 namespace {
 constexpr int NT = 256;
 
-// One block a row at a time, the row read again from the cache for each of its sums.
+// ---------------------------------------------------------------------------------------------- vectors of a row
+template <typename T, int N>
+struct Raw {
+  T v[N];
+};
+template <typename T, int N>
+__device__ __forceinline__ Raw<T, N> load(const T* p) {
+  Raw<T, N> r;
+  __builtin_memcpy(&r, p, sizeof(r));
+  return r;
+}
+template <typename T, int N>
+__device__ __forceinline__ void store(T* p, const float* from) {
+  Raw<T, N> r;
+#pragma unroll
+  for (int i = 0; i < N; i++) r.v[i] = from_f32<T>(from[i]);
+  __builtin_memcpy(p, &r, sizeof(r));
+}
+// N of a parameter's elements; `other` for all where there is none
+template <typename P, int N>
+__device__ __forceinline__ void load_param(const P* p, int at, float other, float* to) {
+  if (p) {
+    const Raw<P, N> r = load<P, N>(p + at);
+#pragma unroll
+    for (int i = 0; i < N; i++) to[i] = to_f32(r.v[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i++) to[i] = other;
+  }
+}
+
+// ---------------------------------------------------------------------------------------------- rows beyond 16384
+// One block a row, the row read again (from the cache) for each of its sums.  Vectors as below: whole, the last one moved back
+// to the row's end; `skip` of its elements are another thread's too.
+constexpr int WT = 1024;
+template <typename T, typename F>
+__device__ __forceinline__ void each_vector(int cols, F&& f) {
+  constexpr int N = 16 / (int)sizeof(T);
+  for (int c = threadIdx.x * N; c < cols; c += WT * N) {
+    const int at = c < cols - N ? c : cols - N;
+    f(at, c - at);
+  }
+}
+
 template <typename T, typename P>
-__global__ __launch_bounds__(NT) void norm_fwd_wide(const T* x, int64_t x_stride, const P* weight, const P* bias, T* y, float* mean_out,
+__global__ __launch_bounds__(WT) void norm_fwd_wide(const T* x, int64_t x_stride, const P* weight, const P* bias, T* y, float* mean_out,
                                                     float* rstd_out, int64_t rows, int cols, float eps) {
-  __shared__ float buf[2][NT / 64];
+  constexpr int N = 16 / (int)sizeof(T);
+  __shared__ float buf[2][WT / 64];
   for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
     const T* xr = x + r * x_stride;
-    T* yr = y + r * (int64_t)cols;
     float s = 0;
-    for (int c = threadIdx.x; c < cols; c += NT) s += to_f32(xr[c]);
-    const float mean = block_sum<NT>(s, buf[0]) / (float)cols;
+    each_vector<T>(cols, [&](int at, int skip) {
+      const Raw<T, N> v = load<T, N>(xr + at);
+#pragma unroll
+      for (int i = 0; i < N; i++) s += i >= skip ? to_f32(v.v[i]) : 0.0f;
+    });
+    const float mean = block_sum<WT>(s, buf[0]) / (float)cols;
     s = 0;
-    for (int c = threadIdx.x; c < cols; c += NT) {
-      const float d = to_f32(xr[c]) - mean;
-      s += d * d;
-    }
-    const float rstd = 1.0f / sqrtf(block_sum<NT>(s, buf[1]) / (float)cols + eps);
-    for (int c = threadIdx.x; c < cols; c += NT) {
-      const float h = (to_f32(xr[c]) - mean) * rstd;
-      yr[c] = from_f32<T>(h * (weight ? to_f32(weight[c]) : 1.0f) + (bias ? to_f32(bias[c]) : 0.0f));
-    }
+    each_vector<T>(cols, [&](int at, int skip) {
+      const Raw<T, N> v = load<T, N>(xr + at);
+#pragma unroll
+      for (int i = 0; i < N; i++) {
+        const float d = to_f32(v.v[i]) - mean;
+        s += i >= skip ? d * d : 0.0f;
+      }
+    });
+    const float rstd = 1.0f / sqrtf(block_sum<WT>(s, buf[1]) / (float)cols + eps);
+    each_vector<T>(cols, [&](int at, int) {
+      const Raw<T, N> v = load<T, N>(xr + at);
+      float w[N], b[N];
+      load_param<P, N>(weight, at, 1.0f, w);
+      load_param<P, N>(bias, at, 0.0f, b);
+#pragma unroll
+      for (int i = 0; i < N; i++) b[i] += (to_f32(v.v[i]) - mean) * rstd * w[i];
+      store<T, N>(y + r * (int64_t)cols + at, b);
+    });
     if (mean_out && threadIdx.x == 0) {
       mean_out[r] = mean;
       rstd_out[r] = rstd;
@@ -40,26 +96,36 @@ __global__ __launch_bounds__(NT) void norm_fwd_wide(const T* x, int64_t x_stride
 }
 
 template <typename T, typename P>
-__global__ __launch_bounds__(NT) void norm_dx_wide(const T* x, int64_t x_stride, const T* dy, int64_t dy_stride, const P* weight, const float* mean_in,
+__global__ __launch_bounds__(WT) void norm_dx_wide(const T* x, int64_t x_stride, const T* dy, int64_t dy_stride, const P* weight, const float* mean_in,
                                                    const float* rstd_in, T* dx, int64_t rows, int cols) {
-  __shared__ float buf[2][NT / 64];
+  constexpr int N = 16 / (int)sizeof(T);
+  __shared__ float buf[2][WT / 64];
   for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
     const T* xr = x + r * x_stride;
     const T* gr = dy + r * dy_stride;
     const float mean = mean_in[r], rstd = rstd_in[r];
     float sg = 0, sgh = 0;
-    for (int c = threadIdx.x; c < cols; c += NT) {
-      const float g = to_f32(gr[c]) * (weight ? to_f32(weight[c]) : 1.0f);
-      sg += g;
-      sgh += g * ((to_f32(xr[c]) - mean) * rstd);
-    }
-    sg = block_sum<NT>(sg, buf[0]) / (float)cols;
-    sgh = block_sum<NT>(sgh, buf[1]) / (float)cols;
-    for (int c = threadIdx.x; c < cols; c += NT) {
-      const float g = to_f32(gr[c]) * (weight ? to_f32(weight[c]) : 1.0f);
-      const float h = (to_f32(xr[c]) - mean) * rstd;
-      dx[r * (int64_t)cols + c] = from_f32<T>(rstd * (g - sg - h * sgh));
-    }
+    each_vector<T>(cols, [&](int at, int skip) {
+      const Raw<T, N> v = load<T, N>(xr + at), d = load<T, N>(gr + at);
+      float w[N];
+      load_param<P, N>(weight, at, 1.0f, w);
+#pragma unroll
+      for (int i = 0; i < N; i++) {
+        const float g = to_f32(d.v[i]) * w[i];
+        sg += i >= skip ? g : 0.0f;
+        sgh += i >= skip ? g * ((to_f32(v.v[i]) - mean) * rstd) : 0.0f;
+      }
+    });
+    sg = block_sum<WT>(sg, buf[0]) / (float)cols;
+    sgh = block_sum<WT>(sgh, buf[1]) / (float)cols;
+    each_vector<T>(cols, [&](int at, int) {
+      const Raw<T, N> v = load<T, N>(xr + at), d = load<T, N>(gr + at);
+      float w[N];
+      load_param<P, N>(weight, at, 1.0f, w);
+#pragma unroll
+      for (int i = 0; i < N; i++) w[i] = rstd * (to_f32(d.v[i]) * w[i] - sg - (to_f32(v.v[i]) - mean) * rstd * sgh);
+      store<T, N>(dx + r * (int64_t)cols + at, w);
+    });
     __syncthreads();
   }
 }
@@ -98,11 +164,6 @@ __global__ __launch_bounds__(NT) void norm_dparam_wide(const T* x, int64_t x_str
 // border (the hardware loads them from any element), and one that would pass the row's end is moved back to end there.
 // Its first `skip` elements are then another thread's too: they are left out of the sums, and stored twice with the
 // same value.
-template <typename T, int N>
-struct Raw {
-  T v[N];
-};
-
 template <int N, int TPR, int V>
 struct Place {
   int at[V], skip[V];  // where vector j starts; its elements that are not this thread's (N: none is)
@@ -116,30 +177,6 @@ struct Place {
   }
 };
 
-template <typename T, int N>
-__device__ __forceinline__ Raw<T, N> load(const T* p) {
-  Raw<T, N> r;
-  __builtin_memcpy(&r, p, sizeof(r));
-  return r;
-}
-template <typename T, int N>
-__device__ __forceinline__ void store(T* p, const float* from) {
-  Raw<T, N> r;
-#pragma unroll
-  for (int i = 0; i < N; i++) r.v[i] = from_f32<T>(from[i]);
-  __builtin_memcpy(p, &r, sizeof(r));
-}
-template <typename P, int N>
-__device__ __forceinline__ void load_param(const P* p, int at, float other, float* to) {
-  if (p) {
-    const Raw<P, N> r = load<P, N>(p + at);
-#pragma unroll
-    for (int i = 0; i < N; i++) to[i] = to_f32(r.v[i]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < N; i++) to[i] = other;
-  }
-}
 // f(i) added up over the elements that are this thread's
 template <int N, typename F>
 __device__ __forceinline__ float own_sum(int skip, F&& f) {
@@ -414,7 +451,7 @@ void forward(const fm_layer_norm_args& a) {
   hipStream_t st = (hipStream_t)a.stream;
   const int cols = (int)a.cols;
   if (cols > WIDEST) {
-    norm_fwd_wide<T, P><<<(int)(a.rows < (1 << 20) ? a.rows : 1 << 20), NT, 0, st>>>((const T*)a.x, a.x_stride, (const P*)a.weight, (const P*)a.bias, (T*)a.y,
+    norm_fwd_wide<T, P><<<(int)(a.rows < (1 << 20) ? a.rows : 1 << 20), WT, 0, st>>>((const T*)a.x, a.x_stride, (const P*)a.weight, (const P*)a.bias, (T*)a.y,
                                                                                      a.mean, a.rstd, a.rows, cols, (float)a.eps);
     return;
   }
@@ -434,7 +471,7 @@ void backward(const fm_layer_norm_args& a) {
   int parts = 0;
   if (a.rows > 0 && cols > WIDEST) {
     if (a.dx)
-      norm_dx_wide<T, P><<<(int)(a.rows < (1 << 20) ? a.rows : 1 << 20), NT, 0, st>>>((const T*)a.x, a.x_stride, (const T*)a.dy, a.dy_stride, (const P*)a.weight,
+      norm_dx_wide<T, P><<<(int)(a.rows < (1 << 20) ? a.rows : 1 << 20), WT, 0, st>>>((const T*)a.x, a.x_stride, (const T*)a.dy, a.dy_stride, (const P*)a.weight,
                                                                                       a.mean, a.rstd, (T*)a.dx, a.rows, cols);
     parts = wide_parts(a.rows);
     if (sums)

@@ -404,6 +404,8 @@ struct Steps {
   // never falls as v falls; -1 above the steps, the last step takes all that lies below
   __device__ __forceinline__ static int of(double t) { return (int)floor(fmin(fmax(t, -1.0), (double)(BINS - 1))); }
   __device__ __forceinline__ int operator()(float v) const { return of(at(v)); }
+  // whether all that the last step holds weighs less than 2^-47 of the row's largest: nothing
+  __device__ __forceinline__ bool past() const { return (BINS - 1 - HEAD) * width >= 33.0; }
   // all logits of steps b0 .. b1 (and a few others) lie within `half` of `mid`
   __device__ __forceinline__ void around(int b0, int b1, float& mid, float& half) const {
     const double d0 = (double)(HEAD - b0) / scale, d1 = (double)(HEAD - b1 - 1) / scale;
@@ -415,7 +417,7 @@ struct Steps {
 
 template <int NT>
 struct Long {
-  static constexpr int LISTED = NT;
+  static constexpr int LISTED = NT == 1024 ? 2048 : 1024;  // categories of one list (with the rest, within 64 KB)
   List<LISTED> l;
   unsigned long long weight[BINS + 1];
   uint32_t count[BINS + 1];
@@ -432,6 +434,7 @@ struct Long {
   Row o;
   Steps steps;
 };
+static_assert(sizeof(Long<1024>) < 64000 && sizeof(Long<256>) < 64000, "dynamic LDS of a launch");
 template <int NT>
 __device__ __forceinline__ Long<NT>& shared() {
   extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
@@ -465,7 +468,7 @@ __device__ __forceinline__ uint64_t block_before(uint64_t mine, unsigned long lo
 template <int NT, bool COUNT, bool WEIGH, typename S>
 __device__ __forceinline__ void weigh_steps(const S& src, const Steps& steps, double one, Long<NT>& g, float& top, int& categories, int& seen) {
   constexpr double LOW = BINS - 1;
-  const bool far = (BINS - 1 - HEAD) * steps.width < 33.0;  // whether the last step can still weigh 2^-46 or more
+  const bool far = !steps.past();
   // exp(-r width) = 1 + r (c1 + r (c2 + r (c3 + r c4))), exact at r = 0: its series with the term of r^5 put into the lower
   // ones by r^4 = 2 r^3 - 5/4 r^2 + r/4 - 1/128, which Chebyshev's polynomial of degree 4 on 0 .. 1 gives to 1/128; 5e-13 in all.
   // In units of 2^-s, and with 2^52 added, which leaves the whole number in the low bits
@@ -699,12 +702,13 @@ __device__ __forceinline__ uint64_t draw_by_steps(const Steps& steps, float top,
   const bool cut = counted && (uint64_t)o.top_k < n;
   uint64_t sum = all;
   if (counted && !weighed) {  // top_k, and few: one list of all that it keeps (of all, where there are fewer)
-    const int to = cut ? step_of(g, g.count, (uint64_t)o.top_k - 1) : BINS - 1;
+    int to = cut ? step_of(g, g.count, (uint64_t)o.top_k - 1) : BINS - 1;
+    if (to == BINS - 1 && steps.past()) to--;  // what lies below weighs nothing
     if (!list_steps<T, MASKED, NT>(0, to, 0, -1)) return 0;
     return draw_from<NT>(g.l, g.listed, o);
   }
-  if (cut) {
-    const int b = step_of(g, g.count, (uint64_t)o.top_k - 1);
+  const int b = cut ? step_of(g, g.count, (uint64_t)o.top_k - 1) : BINS - 1;
+  if (cut && !(b == BINS - 1 && steps.past())) {
     if (!list_steps<T, MASKED, NT>(b, b, 0, -1)) return 0;
     const int i = (int)(o.top_k - 1 - g.count[b]);
     sum = g.weight[b] + g.l.upto[i < g.listed ? i : g.listed - 1];
@@ -836,7 +840,7 @@ __global__ __launch_bounds__(NT, 4) void sample_long(const T* logits, int64_t st
     first = fmaxf(first, g.fbuf[0][w]);
     least = fminf(least, g.fbuf[1][w]);
   }
-  const bool counted = o.top_k > 0 && o.top_k < cols, weighed = !counted || o.top_k > NT / 2;
+  const bool counted = o.top_k > 0 && o.top_k < cols, weighed = !counted || o.top_k > Long<NT>::LISTED / 2;
   for (int turn = 0; turn < 2; turn++) {
     // a power of two of the weight in 32 steps; narrower where the first vectors all lie within 1024 of them
     // T counts as 2^-35 |first| at least: the next float32 below would still weigh e^-2048, and first * scale stays below 2^41
@@ -859,10 +863,11 @@ __global__ __launch_bounds__(NT, 4) void sample_long(const T* logits, int64_t st
     int categories = 0;
     if (!(first > -INFINITY && first < INFINITY)) {  // nothing to start from, or nothing but infinity counts
       seen = 2;
-      src.template each<NT>([&](int, float v) {
+      for (int c = threadIdx.x; c < cols; c += NT) {
+        const float v = src(c);
         seen |= v != v;
         top = fmaxf(top, v);
-      });
+      }
     } else if (!weighed) {
       weigh_steps<NT, true, false>(src, steps, o.one, g, top, categories, seen);
     } else if (!counted) {
@@ -976,7 +981,7 @@ void launch(const fm_sample_args& a) {
     sample_list<T, MASKED, 256, 1024><<<each, 256, 0, st>>>(ARGS);
   else if (cols <= 2048)
     sample_list<T, MASKED, 512, 2048><<<each, 512, 0, st>>>(ARGS);
-  else if (a.rows >= 1024 || cols <= 4096)
+  else if (cols <= 4096 || (a.rows >= 1024 && cols <= 65536))
     sample_long<T, MASKED, 256><<<each, 256, sizeof(Long<256>), st>>>(ARGS);
   else
     sample_long<T, MASKED, 1024><<<each, 1024, sizeof(Long<1024>), st>>>(ARGS);
