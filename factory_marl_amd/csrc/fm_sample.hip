@@ -129,6 +129,7 @@ typedef uint32_t Vec4 __attribute__((aligned(1)));
 template <typename T, bool MASKED>
 struct Source {
   static constexpr int N = 16 / (int)sizeof(T);
+  typedef typename std::conditional<N == 8, Vec8, Vec4>::type Bytes;
   const GLOBAL T* z;
   const GLOBAL uint8_t* mask;
   int cols;
@@ -139,7 +140,6 @@ struct Source {
   // what is left at the end
   template <int NT, int U, typename F, typename G>
   __device__ __forceinline__ void vectors(F&& f, G&& g) const {
-    typedef typename std::conditional<N == 8, Vec8, Vec4>::type Bytes;
     const int count = cols / N;
     for (int i = threadIdx.x; i < count; i += NT * U) {
       Vec16 v[U];
@@ -345,43 +345,231 @@ __device__ uint64_t draw_from(List<LN>& l, int n, const Row& o) {
   return l.place[first_over<NT>(l, kept, target_of(o.u, l.upto[kept - 1]))];
 }
 
-// Rows of at most LN categories, a block each: the whole row is the list.
-template <typename T, bool MASKED, int NT, int LN>
-__global__ __launch_bounds__(NT) void sample_list(const T* logits, int64_t stride, const uint8_t* mask, int64_t mask_stride, Settings a, int64_t* out,
-                                                  int64_t rows, int cols) {
-  __shared__ List<LN> l;
-  __shared__ float fbuf[NT / 64];
-  const int64_t r = blockIdx.x + (int64_t)gridDim.x * blockIdx.y;
-  if (r < rows) {
-    const Source<T, MASKED> src{(const GLOBAL T*)(logits + r * stride), (const GLOBAL uint8_t*)(MASKED ? mask + r * mask_stride : nullptr), cols};
-    const Row o = uniform(row_settings(a, r));
-    for (int c = threadIdx.x; c < cols; c += NT) l.place[c] = 0;
-    __syncthreads();
-    float top = -INFINITY;
-    int wrong = o.nan, n = 0;
-    auto one = [&](int c, float v) {
-      wrong |= v != v;
-      top = fmaxf(top, v);
-      n += v != -INFINITY;
-      if (v != -INFINITY) l.place[c] = place_of(v, c);
-    };
-    src.template vectors<NT, 1>(
-        [&](int c, const float* v) {
+// ---------------------------------------------------------------------------------------------- up to 2048 categories
+// A wave a row, R logits a lane in registers, no barriers.  Weights go to 256 steps of the logit in LDS; the step in which a sum
+// passes a number is found by the lanes' running sums, and its categories, at most 64 as a rule, are compared with each
+// other, one a lane.
+constexpr int WBINS = 256;
+
+__device__ __forceinline__ uint64_t read_lane(uint64_t v, int lane) {
+  return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)v, lane);
+}
+
+template <typename T, bool MASKED, int R>
+struct WaveRow {
+  static constexpr int N = 16 / (int)sizeof(T), V = R / N;
+  struct Lds {
+    unsigned long long weight[WBINS], place[64];
+    uint32_t count[WBINS];
+    int listed;
+  };
+  float x[V][N];
+  float top, scale;
+  int lane;
+  uint64_t wbefore, wbin[WBINS / 64];  // this lane's steps: the weight of all before, and each one's
+  uint32_t cbefore, cbin[WBINS / 64];
+
+  // f(column, logit) over the lane's categories, -inf where one is barred
+  template <typename F>
+  __device__ __forceinline__ void each(F&& f) const {
 #pragma unroll
-          for (int i = 0; i < src.N; i++) one(c + i, v[i]);
-        },
-        one);
-    top = block_max<NT>(top, fbuf);
-    wrong = __syncthreads_or(wrong);
-    n = block_sum<NT>(n, (int*)l.wave);
-    __syncthreads();
-    uint64_t found = 0;
-    if (!wrong && n > 0) {
-      sort_list<NT>(l, cols, top, o);
-      found = draw_from<NT>(l, n, o);
-    }
-    if (threadIdx.x == 0) out[r] = found ? column_of(found) : -1;
+    for (int i = 0; i < V; i++)
+#pragma unroll
+      for (int n = 0; n < N; n++) {
+        f((i * 64 + lane) * N + n, x[i][n]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
   }
+  __device__ __forceinline__ int step_of(float v) const {
+    const float d = v == top ? 0.0f : (top - v) * scale;
+    return d < (float)(WBINS - 1) ? (int)d : WBINS - 1;
+  }
+  // the step in which the running sum passes `number`, and that sum before it (by_count: of ones; wsum: of weights)
+  __device__ __forceinline__ int find_step(bool by_count, uint64_t number, uint64_t& sum, uint64_t& wsum) const {
+    uint64_t s = by_count ? cbefore : wbefore, w = wbefore, at_s = 0, at_w = 0;
+    int found = -1;
+#pragma unroll
+    for (int k = 0; k < WBINS / 64; k++) {
+      const uint64_t own = by_count ? (uint64_t)cbin[k] : wbin[k];
+      if (s <= number && number < s + own) {
+        found = lane * (WBINS / 64) + k;
+        at_s = s;
+        at_w = w;
+      }
+      s += own;
+      w += wbin[k];
+    }
+    const int l = __ffsll((unsigned long long)__ballot(found >= 0)) - 1;
+    sum = read_lane(at_s, l);
+    wsum = read_lane(at_w, l);
+    return __builtin_amdgcn_readlane(found, l);
+  }
+  // The category at which the running sum (of ones, or of weights) passes `number`: its place, and the weight up to and with it.
+  __device__ __forceinline__ uint64_t find(bool by_count, uint64_t number, Lds& g, const Row& o, uint64_t& upto) const {
+    uint64_t sum, wsum;
+    const int step = find_step(by_count, number, sum, wsum);
+    if (lane == 0) g.listed = 0;
+    wave_sync();
+    each([&](int c, float v) {
+      if (v > -INFINITY && step_of(v) == step) {
+        const int i = atomicAdd(&g.listed, 1);
+        if (i < 64) g.place[i] = place_of(v, c);
+      }
+    });
+    wave_sync();
+    const int n = uniform(g.listed);
+    if (n <= 64) {
+      const uint64_t p = lane < n ? g.place[lane] : 0, w = p ? weight_of(logit_of(p), top, o) : 0;
+      uint64_t own = 0, ownw = wsum;  // up to and with this lane's
+      for (int k = 0; k < n; k++) {
+        const bool over = read_lane(p, k) >= p;
+        own += over;
+        ownw += over ? read_lane(w, k) : 0;
+      }
+      own = by_count ? sum + own : ownw;
+      // the first one over the number: of those, the one with the largest place (the last of all, should rounding leave none)
+      uint64_t best = p && own > number ? p : 0;
+      best = sort_lanes<64>(best, lane);
+      best = read_lane(best, 0);
+      const uint64_t hit = __ballot(p && p == best);
+      const int l = hit ? __ffsll((unsigned long long)hit) - 1 : 0;
+      if (best) {
+        upto = read_lane(ownw, l);
+        return best;
+      }
+      uint64_t last = sort_lanes<64>(p ? ~p : 0, lane);
+      last = ~read_lane(last, 0);
+      upto = read_lane(ownw, __ffsll((unsigned long long)__ballot(p == last)) - 1);
+      return last;
+    }
+    // more: bit by bit of its place, the largest one up to which the row's sum is over the number
+    uint64_t place = 0, total = 0;
+    for (int bit = 63; bit >= 0; bit--) {
+      const uint64_t test = place | 1ull << bit;
+      uint64_t s = 0, w = 0;
+      each([&](int c, float v) {
+        if (v > -INFINITY && place_of(v, c) >= test) {
+          const uint64_t own = weight_of(v, top, o);
+          w += own;
+          s += by_count ? 1 : own;
+        }
+      });
+      s = group_sum<64>(s);
+      w = group_sum<64>(w);
+      if (s > number) {
+        place = test;
+        total = w;
+      }
+    }
+    upto = total;
+    return place;
+  }
+};
+
+template <typename T, bool MASKED, int R>
+__global__ __launch_bounds__(256, R > 16 ? 2 : 4) void sample_wave(const T* logits, int64_t stride, const uint8_t* mask, int64_t mask_stride, Settings a, int64_t* out,
+                                                                 int64_t rows, int cols) {
+  typedef WaveRow<T, MASKED, R> W;
+  constexpr int N = W::N;
+  __shared__ typename W::Lds lds[4];
+  const int64_t r = ((int64_t)blockIdx.x + (int64_t)gridDim.x * blockIdx.y) * 4 + uniform((int)(threadIdx.x >> 6));
+  if (r >= rows) return;
+  typename W::Lds& g = lds[threadIdx.x >> 6];
+  const Row o = uniform(row_settings(a, r));
+  W w;
+  w.lane = threadIdx.x & 63;
+  const Source<T, MASKED> src{(const GLOBAL T*)(logits + r * stride), (const GLOBAL uint8_t*)(MASKED ? mask + r * mask_stride : nullptr), cols};
+#pragma unroll
+  for (int i = 0; i < W::V; i++) {  // whole vectors; the row's last elements one at a time
+    const int c = (i * 64 + w.lane) * N;
+    Vec16 v;
+    typename Source<T, MASKED>::Bytes m;
+    const bool whole = c + N <= cols;
+    if (whole) {
+      v = *(const GLOBAL Vec16*)(src.z + c);
+      if (MASKED) m = *(const GLOBAL typename Source<T, MASKED>::Bytes*)(src.mask + c);
+    }
+    T raw[N];
+    uint8_t open[N];
+    __builtin_memcpy(raw, &v, 16);
+    if (MASKED) __builtin_memcpy(open, &m, N);
+#pragma unroll
+    for (int n = 0; n < N; n++) w.x[i][n] = whole && !(MASKED && !open[n]) ? to_f32(raw[n]) : -INFINITY;
+    if (!whole && c < cols)
+#pragma unroll
+      for (int n = 0; n < N; n++)
+        if (c + n < cols) w.x[i][n] = src(c + n);
+  }
+  float top = -INFINITY, least = INFINITY;
+  int wrong = 0;
+  uint32_t n = 0;
+  w.each([&](int, float v) {
+    wrong |= v != v;
+    n += v > -INFINITY;
+    top = fmaxf(top, v);
+    least = fminf(least, v > -INFINITY ? v : INFINITY);
+  });
+  w.top = uniform(group_max<64>(top));
+  least = -group_max<64>(-least);
+  uint64_t found = 0;
+  if (!__ballot(wrong) && !o.nan && w.top > -INFINITY) {
+    if (o.greedy) {
+      w.each([&](int c, float v) {
+        const uint64_t p = v == w.top ? place_of(v, c) : 0;
+        found = p > found ? p : found;
+      });
+      found = read_lane(sort_lanes<64>(found, w.lane), 0);
+    } else {
+      // steps down to weights of e^-32 (with a T of next to nothing, to what float32 can tell apart), or to the row's least logit
+      const float range = w.top - least, reach = fminf(range, fmaxf((float)(32.0 / o.inv_t), range / 4096.0f));
+      w.scale = uniform(reach > 0 ? fminf((float)WBINS / reach, 3e38f) : 0.0f);
+      const bool counted = o.top_k > 0 && o.top_k < cols;
+#pragma unroll
+      for (int k = 0; k < WBINS / 64; k++) {
+        g.weight[k * 64 + w.lane] = 0;
+        g.count[k * 64 + w.lane] = 0;
+      }
+      wave_sync();
+      uint64_t heavy = 0;  // the weight of those that min_p keeps: a leading part, like every setting's
+      w.each([&](int, float v) {
+        if (v == -INFINITY) return;
+        const int b = w.step_of(v);
+        const uint64_t own = weight_of(v, w.top, o);
+        atomicAdd(&g.weight[b], (unsigned long long)own);
+        if (counted) atomicAdd(&g.count[b], 1u);
+        heavy += (double)own >= o.min_w ? own : 0;
+      });
+      wave_sync();
+      uint64_t sum = 0;
+      uint32_t sumc = 0;
+#pragma unroll
+      for (int k = 0; k < WBINS / 64; k++) {
+        w.wbin[k] = g.weight[w.lane * (WBINS / 64) + k];
+        w.cbin[k] = g.count[w.lane * (WBINS / 64) + k];
+        sum += w.wbin[k];
+        sumc += w.cbin[k];
+      }
+      uint64_t all = sum_lanes<64>(sum, w.lane);
+      const uint32_t allc = sum_lanes<64>(sumc, w.lane);
+      w.wbefore = all - sum;
+      w.cbefore = allc - sumc;
+      sum = read_lane(all, 63);
+      n = __builtin_amdgcn_readlane(allc, 63);
+      const bool cut = counted && (uint64_t)o.top_k < n;
+#pragma unroll 1
+      for (int stage = 0; stage < 3; stage++) {  // top_k's border, top_p's, the draw
+        if ((stage == 0 && !cut) || (stage == 1 && o.top_p >= 1)) continue;
+        if (stage == 2 && o.min_w > 0) {
+          const uint64_t kept = group_sum<64>(heavy);
+          sum = kept < sum ? kept : sum;
+        }
+        uint64_t upto;
+        found = w.find(stage == 0, stage == 0 ? (uint64_t)o.top_k - 1 : stage == 1 ? border_of(o.top_p, sum) : target_of(o.u, sum), g, o, upto);
+        sum = upto < sum ? upto : sum;
+      }
+    }
+  }
+  if (w.lane == 0) out[r] = found ? column_of(found) : -1;
 }
 
 // ---------------------------------------------------------------------------------------------- longer rows
@@ -948,8 +1136,8 @@ int shift_of(int64_t cols) {  // the sum of cols weights of at most 2^s stays be
   return s;
 }
 
-// Up to 64 categories a group of lanes holds a row; up to 2048 a block sorts it whole (fewer threads for fewer
-// categories: their barriers cost more than the idle lanes); longer rows are narrowed down first.
+// Up to 64 categories a group of lanes holds a row, up to 2048 a wave, longer rows take a block: of 256 threads (four to a
+// CU) where that fills the chip or the row has little for more, else of 1024.
 template <typename T, bool MASKED>
 void launch(const fm_sample_args& a) {
   const Settings s{a.temperature, a.top_p, a.min_p, a.top_k, a.temperature_rows, a.top_p_rows, a.min_p_rows, a.top_k_rows, a.u, a.u_dtype == FM_DTYPE_F64, shift_of(a.cols)};
@@ -959,6 +1147,7 @@ void launch(const fm_sample_args& a) {
     const int64_t n = (a.rows + rows_each - 1) / rows_each;
     return (int)(n < (1 << 20) ? n : 1 << 20);
   };
+  const dim3 fours(blocks(4), (unsigned)((a.rows + (1 << 22) - 1) >> 22));
   const dim3 each(blocks(1), (unsigned)((a.rows + (1 << 20) - 1) >> 20));
 #define ARGS (const T*)a.logits, a.stride, a.mask, a.mask_stride, s, a.out, a.rows, cols
   if (cols <= 2)
@@ -973,14 +1162,12 @@ void launch(const fm_sample_args& a) {
     sample_group<T, 32><<<blocks(8), 256, 0, st>>>(ARGS);
   else if (cols <= 64)
     sample_group<T, 64><<<blocks(4), 256, 0, st>>>(ARGS);
-  else if (cols <= 256)
-    sample_list<T, MASKED, 64, 256><<<each, 64, 0, st>>>(ARGS);
   else if (cols <= 512)
-    sample_list<T, MASKED, 128, 512><<<each, 128, 0, st>>>(ARGS);
+    sample_wave<T, MASKED, 8><<<fours, 256, 0, st>>>(ARGS);
   else if (cols <= 1024)
-    sample_list<T, MASKED, 256, 1024><<<each, 256, 0, st>>>(ARGS);
+    sample_wave<T, MASKED, 16><<<fours, 256, 0, st>>>(ARGS);
   else if (cols <= 2048)
-    sample_list<T, MASKED, 512, 2048><<<each, 512, 0, st>>>(ARGS);
+    sample_wave<T, MASKED, 32><<<fours, 256, 0, st>>>(ARGS);
   else if (cols <= 4096 || (a.rows >= 1024 && cols <= 65536))
     sample_long<T, MASKED, 256><<<each, 256, sizeof(Long<256>), st>>>(ARGS);
   else
