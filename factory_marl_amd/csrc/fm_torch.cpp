@@ -1,0 +1,232 @@
+// fm_torch.cpp -- the differentiable operators as autograd nodes: factory_marl_amd/ops.py checks and shapes the arguments and calls
+// torch.ops.factorysim.*, whose backward passes run here without the interpreter (a Python node waits for it on the
+// engine's thread: a layer norm of 64 x 128, forward and backward, took 105 us of host time with one and takes 60 like this).
+// All computing is the library's; its entry points are handed over once, by `bind`.
+#include <ATen/ATen.h>
+#include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
+#include <torch/csrc/autograd/saved_variable.h>
+#include <torch/library.h>
+
+#include "../../include/factorysim.h"
+
+namespace {
+using at::Tensor;
+using torch::autograd::SavedVariable;
+using torch::autograd::variable_list;
+
+struct Entries {
+  decltype(&fm_layer_norm_forward) norm_forward;
+  decltype(&fm_layer_norm_backward) norm_backward;
+  decltype(&fm_layer_norm_workspace) norm_workspace;
+  decltype(&fm_distill_forward) distill_forward;
+  decltype(&fm_distill_backward) distill_backward;
+  decltype(&fm_distill_workspace) distill_workspace;
+  decltype(&fm_last_error) last_error;
+} fm;
+
+void bind(at::IntArrayRef addresses) {
+  TORCH_CHECK(addresses.size() * sizeof(void*) == sizeof(fm), "factorysim: entry points");
+  std::memcpy(&fm, addresses.data(), sizeof(fm));
+}
+
+void check(int rc) { TORCH_CHECK(rc == 0, "factorysim error ", rc, ": ", fm.last_error()); }
+
+int32_t code(const Tensor& t) {
+  switch (t.scalar_type()) {
+    case at::kFloat: return FM_DTYPE_F32;
+    case at::kHalf: return FM_DTYPE_F16;
+    case at::kBFloat16: return FM_DTYPE_BF16;
+    case at::kInt: return FM_DTYPE_I32;
+    case at::kLong: return FM_DTYPE_I64;
+    default: TORCH_CHECK_TYPE(false, "factorysim: element type ", t.scalar_type());
+  }
+}
+
+// device and stream of a call on t: the current stream of its device, which inside a backward pass the engine has set to the
+// forward pass's
+template <typename Args>
+void place(Args& a, const Tensor& t) {
+  a.device = t.is_cpu() ? -1 : (int32_t)t.device().index();
+  a.stream = t.is_cpu() ? nullptr : (void*)c10::hip::getCurrentHIPStream(t.device().index()).stream();
+}
+
+int64_t row_stride(const Tensor& t) { return t.size(0) > 1 ? t.stride(0) : 0; }
+void* data(const Tensor& t) { return t.defined() && t.numel() ? t.data_ptr() : nullptr; }
+
+// [rows, cols] with adjacent columns
+Tensor rows_of(const Tensor& t) { return t.size(1) <= 1 || t.stride(1) == 1 ? t : t.contiguous(); }
+
+template <typename Args>
+Tensor workspace(Args& a, int64_t bytes, const Tensor& like) {
+  if (a.device < 0 || bytes <= 0) return Tensor();
+  Tensor t = at::empty({bytes}, like.options().dtype(at::kByte));
+  a.workspace = data(t);
+  a.workspace_bytes = bytes;
+  return t;
+}
+
+// a backward pass's results; differentiating them is refused, where a graph of them is being made
+variable_list once(variable_list out) {
+  if (!at::GradMode::is_enabled()) return out;
+  auto refuse = std::make_shared<torch::autograd::DelayedError>("factorysim: this operator is differentiable once", (int)out.size());
+  return (*refuse)(std::move(out));
+}
+
+// ------------------------------------------------------------------ layer norm
+struct LayerNormBackward : public torch::autograd::Node {
+  SavedVariable x, weight, stats;
+  at::ScalarType param;
+
+  variable_list apply(variable_list&& grads) override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    variable_list out(3);
+    if (!grads[0].defined()) return out;
+    const Tensor x_ = x.unpack(), w = weight.unpack(), s = stats.unpack(), dy = rows_of(grads[0]);
+    const auto parameter = x_.options().dtype(param);
+    if (task_should_compute_output(0)) out[0] = at::empty(x_.sizes(), x_.options());
+    if (task_should_compute_output(1)) out[1] = at::empty({x_.size(1)}, parameter);
+    if (task_should_compute_output(2)) out[2] = at::empty({x_.size(1)}, parameter);
+    fm_layer_norm_args a = {};
+    place(a, x_);
+    a.x_dtype = code(x_);
+    a.param_dtype = param == x_.scalar_type() ? a.x_dtype : FM_DTYPE_F32;
+    a.rows = x_.size(0);
+    a.cols = x_.size(1);
+    a.x = data(x_);
+    a.x_stride = row_stride(x_);
+    a.weight = data(w);
+    a.mean = (float*)data(s);
+    a.rstd = a.mean + a.rows;
+    a.dy = data(dy);
+    a.dy_stride = row_stride(dy);
+    a.dx = data(out[0]);
+    a.dweight = data(out[1]);
+    a.dbias = data(out[2]);
+    const Tensor work = workspace(a, out[1].defined() || out[2].defined() ? fm.norm_workspace(a.rows, a.cols) : 0, x_);
+    check(fm.norm_backward(&a));
+    return once(std::move(out));
+  }
+  void release_variables() override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    x.reset_data();
+    weight.reset_data();
+    stats.reset_data();
+  }
+  std::string name() const override { return "LayerNormBackward"; }
+};
+
+// x [rows, cols] with adjacent columns; weight, bias [cols], contiguous
+Tensor layer_norm(const Tensor& x, const std::optional<Tensor>& weight, const std::optional<Tensor>& bias, double eps) {
+  const Tensor w = weight.value_or(Tensor()), b = bias.value_or(Tensor());
+  const bool graph = torch::autograd::compute_requires_grad(x, w, b);
+  const int64_t n = x.size(0);
+  Tensor y = at::empty({n, x.size(1)}, x.options().requires_grad(false)), stats;
+  fm_layer_norm_args a = {};
+  place(a, x);
+  a.x_dtype = code(x);
+  a.param_dtype = w.defined() ? code(w) : b.defined() ? code(b) : a.x_dtype;
+  a.rows = n;
+  a.cols = x.size(1);
+  a.x = data(x);
+  a.x_stride = row_stride(x);
+  a.weight = data(w);
+  a.bias = data(b);
+  a.eps = eps;
+  a.y = data(y);
+  if (graph) {
+    stats = at::empty({2, n}, x.options().dtype(at::kFloat).requires_grad(false));
+    a.mean = (float*)data(stats);
+    a.rstd = n ? a.mean + n : nullptr;
+  }
+  check(fm.norm_forward(&a));
+  if (!graph) return y;
+  auto node = std::shared_ptr<LayerNormBackward>(new LayerNormBackward(), torch::autograd::deleteNode);
+  node->set_next_edges(torch::autograd::collect_next_edges(x, w, b));
+  node->x = SavedVariable(x, false);
+  node->weight = SavedVariable(w, false);
+  node->stats = SavedVariable(stats, false);
+  node->param = w.defined() ? w.scalar_type() : b.defined() ? b.scalar_type() : x.scalar_type();
+  torch::autograd::set_history(y, node);
+  return y;
+}
+
+// ------------------------------------------------------------------ distillation
+fm_distill_args distill_args(const Tensor& z, const Tensor& index, const Tensor& teacher, double temperature) {
+  fm_distill_args a = {};
+  place(a, z);
+  a.dtype = code(z);
+  a.index_dtype = code(index);
+  a.teacher_dtype = code(teacher);
+  a.rows = z.size(0);
+  a.cols = z.size(1);
+  a.k = index.size(1);
+  a.logits = data(z);
+  a.stride = row_stride(z);
+  a.index = data(index);
+  a.index_stride = row_stride(index);
+  a.teacher = data(teacher);
+  a.teacher_stride = row_stride(teacher);
+  a.temperature = temperature;
+  return a;
+}
+
+struct DistillBackward : public torch::autograd::Node {
+  SavedVariable z, index, teacher, stats;
+  double temperature;
+
+  variable_list apply(variable_list&& grads) override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    variable_list out(1);
+    if (!grads[0].defined()) return out;
+    const Tensor z_ = z.unpack(), i = index.unpack(), t = teacher.unpack(), s = stats.unpack(), &g = grads[0];
+    out[0] = at::empty(z_.sizes(), z_.options());
+    fm_distill_args a = distill_args(z_, i, t, temperature);
+    a.stats = (float*)data(s);
+    a.grad = (const float*)data(g);
+    a.grad_stride = row_stride(g);
+    a.dlogits = data(out[0]);
+    check(fm.distill_backward(&a));
+    return once(std::move(out));
+  }
+  void release_variables() override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    z.reset_data();
+    index.reset_data();
+    teacher.reset_data();
+    stats.reset_data();
+  }
+  std::string name() const override { return "DistillBackward"; }
+};
+
+// z [rows, cols], index and teacher [rows, k], all with adjacent columns
+Tensor distill_loss(const Tensor& z, const Tensor& index, const Tensor& teacher, double temperature) {
+  const bool graph = torch::autograd::compute_requires_grad(z);
+  fm_distill_args a = distill_args(z, index, teacher, temperature);
+  const auto floats = z.options().dtype(at::kFloat).requires_grad(false);
+  Tensor loss = at::empty({a.rows}, floats), stats;
+  if (graph) stats = at::empty({a.rows, 2}, floats);
+  a.loss = (float*)data(loss);
+  a.stats = (float*)data(stats);
+  const Tensor work = workspace(a, fm.distill_workspace(a.rows, a.cols), z);
+  check(fm.distill_forward(&a));
+  if (!graph) return loss;
+  auto node = std::shared_ptr<DistillBackward>(new DistillBackward(), torch::autograd::deleteNode);
+  node->set_next_edges(torch::autograd::collect_next_edges(z));
+  node->z = SavedVariable(z, false);
+  node->index = SavedVariable(index, false);
+  node->teacher = SavedVariable(teacher, false);
+  node->stats = SavedVariable(stats, false);
+  node->temperature = temperature;
+  torch::autograd::set_history(loss, node);
+  return loss;
+}
+}  // namespace
+
+TORCH_LIBRARY(factorysim, m) {
+  m.def("bind(int[] addresses) -> ()", &bind);
+  m.def("layer_norm(Tensor x, Tensor? weight, Tensor? bias, float eps) -> Tensor", &layer_norm);
+  m.def("distill_loss(Tensor logits, Tensor teacher_index, Tensor teacher_logits, float temperature) -> Tensor", &distill_loss);
+}

@@ -7,11 +7,12 @@ row stride; one whose last dimension is not adjacent in memory is copied first. 
 calls, so each call, forward or backward, can be captured into a graph.  A backward pass that is captured needs leaves
 that no live eager graph holds: torch ties a leaf's gradient to the stream of the graph that first used it.
 """
+import ctypes as C
 import math
+import os
 
 import torch
 import torch.nn as nn
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 
@@ -20,14 +21,37 @@ __all__ = ["layer_norm", "LayerNorm", "sample_logits", "distill_loss", "MAX_LIST
 MAX_LISTED = _lib.FM_DISTILL_MAX_K  # most categories that distill_loss takes for a row
 
 _DTYPES = {torch.float32: _lib.FM_DTYPE_F32, torch.float16: _lib.FM_DTYPE_F16, torch.bfloat16: _lib.FM_DTYPE_BF16}
-_INDEX = {torch.int32: _lib.FM_DTYPE_I32, torch.int64: _lib.FM_DTYPE_I64}
+_INDEX = (torch.int32, torch.int64)
+
+
+_NODES = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libfactorysim_torch.so")
+_loaded = None
 
 
 def _library():
-    L = _lib.load()
-    if not hasattr(L, "fm_layer_norm_forward"):
-        raise _lib.FactorySimError(f"{_lib.LIB_PATH} has no operators: rebuild it")
-    return L
+    """the library, its differentiable operators registered with torch (csrc/fm_torch.cpp)"""
+    global _loaded
+    if _loaded is None:
+        L = _lib.load()
+        if not hasattr(L, "fm_layer_norm_forward"):
+            raise _lib.FactorySimError(f"{_lib.LIB_PATH} has no operators: rebuild it")
+        if not os.path.exists(_NODES):
+            raise _lib.FactorySimError(f"{_NODES} not built: run `python __graft_entry__.py build`")
+        torch.ops.load_library(_NODES)
+        names = ("fm_layer_norm_forward", "fm_layer_norm_backward", "fm_layer_norm_workspace", "fm_distill_forward",
+                 "fm_distill_backward", "fm_distill_workspace", "fm_last_error")
+        torch.ops.factorysim.bind([C.cast(getattr(L, n), C.c_void_p).value for n in names])
+        _loaded = L
+    return _loaded
+
+
+def _call(op, *args):
+    try:
+        return op(*args)
+    except RuntimeError as e:
+        if "factorysim error" in str(e):
+            raise _lib.FactorySimError(str(e).split("\n")[0]) from None
+        raise
 
 
 def _where(t):
@@ -35,8 +59,6 @@ def _where(t):
     if t.is_cuda:
         d = t.device.index
         return d, torch._C._cuda_getCurrentRawStream(d)
-    if t.device.type != "cpu":
-        raise ValueError(f"tensors are on a GPU or the CPU, not on {t.device}")
     return -1, None
 
 
@@ -59,6 +81,8 @@ def _float_input(name, t):
         raise TypeError(f"{name} is float32, float16 or bfloat16, not {t.dtype}")
     if t.dim() < 1 or t.shape[-1] < 1:
         raise ValueError(f"{name} needs a last dimension of at least 1, got shape {tuple(t.shape)}")
+    if not t.is_cuda and t.device.type != "cpu":
+        raise ValueError(f"{name} is on {t.device}: a GPU or the CPU is needed")
 
 
 def _same_device(t, **others):
@@ -72,52 +96,6 @@ def _ptr(t):
 
 
 # ------------------------------------------------------------------ layer norm
-def _norm_forward(x, weight, bias, eps, keep):
-    L = _library()
-    dev, stream = _where(x)
-    n, v = x.shape
-    y = torch.empty((n, v), dtype=x.dtype, device=x.device)
-    stats = torch.empty((2, n), dtype=torch.float32, device=x.device) if keep else None
-    mean = _ptr(stats)
-    p = weight if weight is not None else bias
-    a = _lib.FmLayerNormArgs(dev, _DTYPES[x.dtype], _DTYPES[x.dtype if p is None else p.dtype], 0, n, v, x.data_ptr(),
-                             _stride(x), _ptr(weight), _ptr(bias), eps, y.data_ptr(), mean,
-                             mean + 4 * n if keep else None, None, 0, None, None, None, None, 0, stream)
-    _lib.check(L.fm_layer_norm_forward(a), L)
-    return y, stats
-
-
-class _LayerNorm(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, eps):
-        y, stats = _norm_forward(x, weight, bias, eps, True)
-        ctx.save_for_backward(x, weight, stats)
-        ctx.bias_dtype = None if bias is None else bias.dtype
-        return y
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        x, weight, stats = ctx.saved_tensors
-        L = _library()
-        dev, stream = _where(x)
-        n, v = x.shape
-        dy = _rows(dy)
-        want_x, want_w, want_b = ctx.needs_input_grad[:3]
-        pt = weight.dtype if weight is not None else ctx.bias_dtype or x.dtype
-        dx = torch.empty((n, v), dtype=x.dtype, device=x.device) if want_x else None
-        dw = torch.empty(v, dtype=pt, device=x.device) if want_w else None
-        db = torch.empty(v, dtype=pt, device=x.device) if want_b else None
-        need = L.fm_layer_norm_workspace(n, v) if (want_w or want_b) and dev >= 0 else 0
-        work = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
-        mean = stats.data_ptr()
-        a = _lib.FmLayerNormArgs(dev, _DTYPES[x.dtype], _DTYPES[pt], 0, n, v, x.data_ptr(), _stride(x), _ptr(weight),
-                                 None, 0.0, None, mean, mean + 4 * n, dy.data_ptr(), _stride(dy), _ptr(dx), _ptr(dw),
-                                 _ptr(db), _ptr(work), need, stream)
-        _lib.check(L.fm_layer_norm_backward(a), L)
-        return dx, dw, db, None
-
-
 def layer_norm(x, weight=None, bias=None, eps=1e-5):
     """(x - mean) / sqrt(variance + eps) * weight + bias over the last dimension (biased variance), in x's dtype.
 
@@ -141,11 +119,8 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
         raise ValueError(f"eps is finite and not negative, got {eps}")
     w = weight if weight is None or weight.is_contiguous() else weight.contiguous()
     b = bias if bias is None or bias.is_contiguous() else bias.contiguous()
-    x2 = _rows(x)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x2, w, b)):
-        y = _LayerNorm.apply(x2, w, b, eps)
-    else:
-        y = _norm_forward(x2, w, b, eps, False)[0]
+    _library()
+    y = _call(torch.ops.factorysim.layer_norm, _rows(x), w, b, eps)
     return y if x.dim() == 2 else y.view(x.shape)
 
 
@@ -199,7 +174,7 @@ def sample_logits(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, mas
     if u.shape != logits.shape[:-1]:
         raise ValueError(f"u has shape {tuple(u.shape)}, the logits' rows {tuple(logits.shape[:-1])}")
     _same_device(logits, u=u, mask=mask, **{n: s for n, s in (("temperature", temperature), ("top_k", top_k),
-                                                               ("top_p", top_p), ("min_p", min_p)) if torch.is_tensor(s)})
+                                                              ("top_p", top_p), ("min_p", min_p)) if torch.is_tensor(s)})
     z = _rows(logits)
     n, v = z.shape
     m = None
@@ -230,47 +205,6 @@ def sample_logits(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, mas
 
 
 # ------------------------------------------------------------------ distillation
-def _distill_args(z, index, teacher, temperature):
-    dev, stream = _where(z)
-    n, v = z.shape
-    return _lib.FmDistillArgs(dev, _DTYPES[z.dtype], _INDEX[index.dtype], _DTYPES[teacher.dtype], n, v, index.shape[1],
-                              z.data_ptr(), _stride(z), index.data_ptr(), _stride(index), teacher.data_ptr(),
-                              _stride(teacher), temperature, None, None, None, 0, None, None, 0, stream)
-
-
-def _distill_forward(z, index, teacher, temperature, keep):
-    L = _library()
-    a = _distill_args(z, index, teacher, temperature)
-    n = z.shape[0]
-    loss = torch.empty(n, dtype=torch.float32, device=z.device)
-    stats = torch.empty((n, 2), dtype=torch.float32, device=z.device) if keep else None
-    need = L.fm_distill_workspace(n, z.shape[1]) if a.device >= 0 else 0
-    work = torch.empty(need, dtype=torch.uint8, device=z.device) if need else None
-    a.loss, a.stats, a.workspace, a.workspace_bytes = loss.data_ptr(), _ptr(stats), _ptr(work), need
-    _lib.check(L.fm_distill_forward(a), L)
-    return loss, stats
-
-
-class _Distill(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, z, index, teacher, temperature):
-        loss, stats = _distill_forward(z, index, teacher, temperature, True)
-        ctx.save_for_backward(z, index, teacher, stats)
-        ctx.temperature = temperature
-        return loss
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad):
-        z, index, teacher, stats = ctx.saved_tensors
-        L = _library()
-        a = _distill_args(z, index, teacher, ctx.temperature)
-        dz = torch.empty(z.shape, dtype=z.dtype, device=z.device)
-        a.stats, a.grad, a.grad_stride, a.dlogits = stats.data_ptr(), grad.data_ptr(), grad.stride(0), dz.data_ptr()
-        _lib.check(L.fm_distill_backward(a), L)
-        return dz, None, None, None
-
-
 def distill_loss(logits, teacher_index, teacher_logits, temperature=1.0):
     """temperature^2 times the Kullback-Leibler divergence of softmax(logits / temperature) over all categories from
     softmax(teacher_logits / temperature) over the listed ones, for each row: float32 [...].
@@ -296,9 +230,6 @@ def distill_loss(logits, teacher_index, teacher_logits, temperature=1.0):
     temperature = float(temperature)
     if not 1e-30 <= temperature <= 1e30:
         raise ValueError(f"temperature is positive and within 1e-30 .. 1e30, got {temperature}")
-    z, index, teacher = _rows(logits), _rows(teacher_index), _rows(teacher_logits)
-    if torch.is_grad_enabled() and z.requires_grad:
-        loss = _Distill.apply(z, index, teacher, temperature)
-    else:
-        loss = _distill_forward(z, index, teacher, temperature, False)[0]
+    _library()
+    loss = _call(torch.ops.factorysim.distill_loss, _rows(logits), _rows(teacher_index), _rows(teacher_logits), temperature)
     return loss if logits.dim() == 2 else loss.view(logits.shape[:-1])
