@@ -719,7 +719,7 @@ __device__ __forceinline__ int step_of(Long<NT>& g, const V* sums, uint64_t numb
   __syncthreads();
   const int b = g.step;
   __syncthreads();
-  return b;
+  return b < 0 ? 0 : b < BINS ? b : BINS - 1;
 }
 
 // Lists and sorts the categories of steps a0 .. a1 and b0 .. b1.  False, for all threads, where they are too many.
@@ -759,6 +759,7 @@ __device__ __noinline__ bool list_steps(int a0, int a1, int b0, int b1) {
       take);
   __syncthreads();
   const int n = uniform(g.listed);
+  __syncthreads();  // all have read it: the next list begins by clearing it
   if (n > Long<NT>::LISTED) return false;
   sort_list<NT>(g.l, n, uniform(g.top), uniform(g.o));
   return true;
@@ -892,14 +893,16 @@ __device__ __forceinline__ uint64_t draw_by_steps(const Steps& steps, float top,
   if (counted && !weighed) {  // top_k, and few: one list of all that it keeps (of all, where there are fewer)
     int to = cut ? step_of(g, g.count, (uint64_t)o.top_k - 1) : BINS - 1;
     if (to == BINS - 1 && steps.past()) to--;  // what lies below weighs nothing
-    if (!list_steps<T, MASKED, NT>(0, to, 0, -1)) return 0;
+    if (!list_steps<T, MASKED, NT>(0, to, 0, -1) || !g.listed) return 0;
     return draw_from<NT>(g.l, g.listed, o);
   }
   const int b = cut ? step_of(g, g.count, (uint64_t)o.top_k - 1) : BINS - 1;
   if (cut && !(b == BINS - 1 && steps.past())) {
     if (!list_steps<T, MASKED, NT>(b, b, 0, -1)) return 0;
     const int i = (int)(o.top_k - 1 - g.count[b]);
+    if (!g.listed) return 0;
     sum = g.weight[b] + g.l.upto[i < g.listed ? i : g.listed - 1];
+    sum = sum < all ? sum : all;  // (the steps' weights and their categories' differ by roundings)
     __syncthreads();
   }
   // the steps of the border behind which nothing is kept: top_p's, or, where it comes first, min_p's (its logit is known
@@ -958,11 +961,15 @@ __device__ __forceinline__ uint64_t draw_by_steps(const Steps& steps, float top,
         }
         const uint64_t kept = base + (end > split ? g.l.upto[end - 1] - off : 0);
         sum = kept < sum ? kept : sum;
+        if (!sum) return 0;
       }
       const uint64_t number = target_of(o.u, sum);
-      if (together) return g.l.place[first_over<NT>(g.l, border && !joined ? split : g.listed, number < tbase ? 0 : number - tbase)];
+      if (together) {
+        const int n = border && !joined ? split : g.listed;
+        return n ? g.l.place[first_over<NT>(g.l, n, number < tbase ? 0 : number - tbase)] : 0;
+      }
       const int b = step_of(g, g.weight, number);
-      if (!list_steps<T, MASKED, NT>(b, b, 0, -1)) return 0;
+      if (!list_steps<T, MASKED, NT>(b, b, 0, -1) || !g.listed) return 0;
       return g.l.place[first_over<NT>(g.l, g.listed, number - g.weight[b])];
     }
   }
@@ -1003,9 +1010,11 @@ __global__ __launch_bounds__(NT, 4) void sample_long(const T* logits, int64_t st
   // the first vectors: where the steps start and how narrow they can be
   const Source<T, MASKED> start{src.z, src.mask, cols < NT * (16 / (int)sizeof(T)) ? cols : NT * (16 / (int)sizeof(T))};
   float first = -INFINITY, least = INFINITY;
+  int open = 0;
   auto look = [&](int, float v) {
     first = fmaxf(first, v);
     least = fminf(least, v > -INFINITY ? v : INFINITY);
+    open += v > -INFINITY;
   };
   start.template vectors<NT, 1>(
       [&](int c, const float* v) {
@@ -1019,21 +1028,26 @@ __global__ __launch_bounds__(NT, 4) void sample_long(const T* logits, int64_t st
   }
   first = group_max<64>(first);
   least = -group_max<64>(-least);
+  open = group_sum<64>(open);
   if ((threadIdx.x & 63) == 0) {
     g.fbuf[0][threadIdx.x >> 6] = first;
     g.fbuf[1][threadIdx.x >> 6] = least;
+    g.wave[threadIdx.x >> 6] = open;
   }
   __syncthreads();
+  open = 0;
   for (int w = 0; w < NT / 64; w++) {
     first = fmaxf(first, g.fbuf[0][w]);
     least = fminf(least, g.fbuf[1][w]);
+    open += (int)g.wave[w];
   }
   const bool counted = o.top_k > 0 && o.top_k < cols, weighed = !counted || o.top_k > Long<NT>::LISTED / 2;
   for (int turn = 0; turn < 2; turn++) {
-    // a power of two of the weight in 32 steps; narrower where the first vectors all lie within 1024 of them
+    // a power of two of the weight in 32 steps; narrower where the first vectors (enough of them that are not barred) lie within 1024
     // T counts as 2^-35 |first| at least: the next float32 below would still weigh e^-2048, and first * scale stays below 2^41
     const double most = 34359738368.0 / fabs((double)first), inv_t = fmin(o.inv_t, most);
-    const double wanted = fmin(fmin(fmax(32.0 * 1.4426950408889634 * inv_t, 1024.0 / ((double)first - (double)least)), 64.0 * most), 1e300);
+    const double close = open < 256 ? 0.0 : 1024.0 / ((double)first - (double)least);
+    const double wanted = fmin(fmin(fmax(fmax(32.0 * 1.4426950408889634 * inv_t, close), 1e-30), 64.0 * most), 1e300);
     Steps steps;
     steps.first = uniform(first);
     steps.scale = uniform(__longlong_as_double(__double_as_longlong(wanted) >> 37 << 37));

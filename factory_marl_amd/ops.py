@@ -141,20 +141,19 @@ class LayerNorm(nn.Module):
 
 
 # ------------------------------------------------------------------ drawing categories
-def _setting(name, value, rows, logits, dtype):
-    """(number, None) or (0, tensor of one number a row)"""
-    if not torch.is_tensor(value):
-        return (int(value) if dtype == torch.int32 else float(value)), None
+def _row_setting(name, value, rows, logits, dtype):
+    """a setting of each row as a contiguous tensor of the library's type"""
     if value.dtype.is_floating_point != (dtype == torch.float32) or value.dtype in (torch.bool, torch.float64):
         raise TypeError(f"{name} of each row is {'a float32' if dtype == torch.float32 else 'an integer'} tensor, not {value.dtype}")
     if value.numel() != rows or (value.dim() > 1 and value.shape != logits.shape[:-1]):
         raise ValueError(f"{name} has shape {tuple(value.shape)}, the logits' rows {tuple(logits.shape[:-1])}")
+    if value.device != logits.device:
+        raise ValueError(f"{name} is on {value.device}, the logits on {logits.device}")
     if value.dtype == torch.int64:  # beyond any number of categories is off, as 0 is
         value = value.clamp(0, 2**31 - 1)
-    return 0, value.reshape(-1).to(dtype).contiguous()
+    return value.reshape(-1).to(dtype).contiguous()
 
 
-@torch.no_grad()
 def sample_logits(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, mask=None):
     """One category of each row of ``logits`` [..., categories], drawn with the uniform numbers ``u`` [...]: int64 [...].
 
@@ -173,9 +172,9 @@ def sample_logits(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, mas
         raise TypeError("u is a float32 or float64 tensor")
     if u.shape != logits.shape[:-1]:
         raise ValueError(f"u has shape {tuple(u.shape)}, the logits' rows {tuple(logits.shape[:-1])}")
-    _same_device(logits, u=u, mask=mask, **{n: s for n, s in (("temperature", temperature), ("top_k", top_k),
-                                                              ("top_p", top_p), ("min_p", min_p)) if torch.is_tensor(s)})
-    z = _rows(logits)
+    if u.device != logits.device:
+        raise ValueError(f"u is on {u.device}, the logits on {logits.device}")
+    z = _rows(logits.detach())
     n, v = z.shape
     m = None
     if mask is not None:
@@ -183,19 +182,27 @@ def sample_logits(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, mas
             raise TypeError(f"mask is a bool tensor, not {mask.dtype}")
         if mask.shape != logits.shape and tuple(mask.shape) != (v,):
             raise ValueError(f"mask has shape {tuple(mask.shape)}, the logits {tuple(logits.shape)}")
+        if mask.device != logits.device:
+            raise ValueError(f"mask is on {mask.device}, the logits on {logits.device}")
         m = _rows(mask if mask.shape == logits.shape else mask[None])
-    t, t_rows = _setting("temperature", temperature, n, logits, torch.float32)
-    k, k_rows = _setting("top_k", top_k, n, logits, torch.int32)
-    p, p_rows = _setting("top_p", top_p, n, logits, torch.float32)
-    q, q_rows = _setting("min_p", min_p, n, logits, torch.float32)
+    t_rows = k_rows = p_rows = q_rows = None
+    if torch.is_tensor(temperature):
+        temperature, t_rows = 0.0, _row_setting("temperature", temperature, n, logits, torch.float32)
+    if torch.is_tensor(top_k):
+        top_k, k_rows = 0, _row_setting("top_k", top_k, n, logits, torch.int32)
+    if torch.is_tensor(top_p):
+        top_p, p_rows = 0.0, _row_setting("top_p", top_p, n, logits, torch.float32)
+    if torch.is_tensor(min_p):
+        min_p, q_rows = 0.0, _row_setting("min_p", min_p, n, logits, torch.float32)
+    t, p, q, k = float(temperature), float(top_p), float(min_p), int(top_k)
     if t != t or p != p or q != q:
         raise ValueError("temperature, top_p and min_p are numbers, not NaN")
-    u = u.reshape(-1).contiguous()
+    u = u.detach().reshape(-1).contiguous() if u.dim() != 1 or not u.is_contiguous() else u
     L = _library()
-    dev, stream = _where(logits)
-    out = torch.empty(logits.shape[:-1], dtype=torch.int64, device=logits.device)
+    dev, stream = _where(z)
+    out = torch.empty(logits.shape[:-1], dtype=torch.int64, device=z.device)
     need = L.fm_sample_workspace(n, v) if dev >= 0 else 0
-    work = torch.empty(need, dtype=torch.uint8, device=logits.device) if need else None
+    work = torch.empty(need, dtype=torch.uint8, device=z.device) if need else None
     a = _lib.FmSampleArgs(dev, _DTYPES[z.dtype], _lib.FM_DTYPE_F32 if u.dtype == torch.float32 else _lib.FM_DTYPE_F64, 0,
                           n, v, z.data_ptr(), _stride(z), _ptr(m), 0 if m is None else _stride(m), u.data_ptr(), t, p,
                           q, min(max(k, 0), 2**31 - 1), _ptr(t_rows), _ptr(p_rows), _ptr(q_rows), _ptr(k_rows), out.data_ptr(),
