@@ -607,8 +607,8 @@ template <int NT>
 struct Long {
   static constexpr int LISTED = NT == 1024 ? 2048 : 1024;  // categories of one list (with the rest, within 64 KB)
   List<LISTED> l;
-  unsigned long long weight[BINS + 1];
-  uint32_t count[BINS + 1];
+  unsigned long long weight[BINS + 1 + 64];
+  uint32_t count[BINS + 1 + 64];
   unsigned long long wave[NT / 64], ubuf[NT / 64];
   unsigned long long place, before, upto;  // find: the category found; the weight before it and with it
   float fbuf[2][NT / 64];
@@ -650,64 +650,60 @@ __device__ __forceinline__ uint64_t block_before(uint64_t mine, unsigned long lo
   return before + run - mine;
 }
 
-// The first pass: counts and / or mantissas of every step.  Returns what only the row as a whole shows: its largest logit,
-// the number of its categories (COUNT), and as bits of `seen` a NaN (1) and a logit above the steps (2).  The last step's
-// count is what the others leave, its weight is g.tail.
+// The first pass: counts and / or mantissas of every step.  Returns what only the row as a whole shows: its largest logit
+// (which tells whether one lay above the steps: those went to step 0, and the pass is made again), the number of its
+// categories (COUNT), and in `seen` a NaN.  The last step's count is what the others leave, its weight is g.tail.
 template <int NT, bool COUNT, bool WEIGH, typename S>
 __device__ __forceinline__ void weigh_steps(const S& src, const Steps& steps, double one, Long<NT>& g, float& top, int& categories, int& seen) {
-  constexpr double LOW = BINS - 1;
-  const bool far = !steps.past();
+  const bool far = WEIGH && !steps.past();
   // exp(-r width) = 1 + r (c1 + r (c2 + r (c3 + r c4))), exact at r = 0: its series with the term of r^5 put into the lower
   // ones by r^4 = 2 r^3 - 5/4 r^2 + r/4 - 1/128, which Chebyshev's polynomial of degree 4 on 0 .. 1 gives to 1/128; 5e-13 in all.
   // In units of 2^-s, and with 2^52 added, which leaves the whole number in the low bits
   const double w = steps.width, e5 = -w * w * w * w * w / 120;
-  const double c1 = uniform(one * (-w - e5 / 128)), c2 = uniform(one * (w * w / 2 + e5 / 4));
-  const double c3 = uniform(one * (-w * w * w / 6 - e5 * 1.25)), c4 = uniform(one * (w * w * w * w / 24 + e5 * 2));
-  const double c0 = uniform(one + 4503599627370496.0);
-  // what lies in the steps; false for what may need a look: above them, NaN, and, where it can weigh, below them
-  auto fast = [&](float v) {
+  const double c1 = uniform(one * (-w - e5 / 128)), c2 = uniform(one * (w * w / 2 + e5 / 4)), c4 = uniform(one * (w * w * w * w / 24 + e5 * 2));
+  // an operation takes one operand from scalar registers: the others stay in vector registers
+  double c3 = one * (-w * w * w / 6 - e5 * 1.25), c0 = one + 4503599627370496.0, base = steps.base;
+  asm volatile("" : "+v"(c3), "+v"(c0), "+v"(base));
+  const uint32_t spare = BINS + 1 + (threadIdx.x & 63);  // where the weight of what lies below the steps goes, each lane's its own
+  auto weigh = [&](float v) {
     top = fmaxf(top, v);
+    seen |= v != v;
     if (COUNT) categories += v > -INFINITY;
-    const double t = steps.at(v);
-    const uint32_t upper = (uint32_t)(__double_as_longlong(t) >> 32);
-    const bool in = upper < 0x409FFC00u;  // 0 <= t < 2047, by its upper word: a sign or NaN makes that larger
-    if (in) {
-      const int b = (int)t;
-      if (COUNT) atomicAdd(&g.count[b], 1u);
-      if (WEIGH) {
-        const double r = __builtin_amdgcn_fract(t);
-        double e = fma(r, c4, c3);
-        e = fma(e, r, c2);
-        e = fma(e, r, c1);
-        e = fma(e, r, c0);
-        atomicAdd(&g.weight[b], (unsigned long long)__double_as_longlong(e) & 0xfffffffffffffull);
-      }
+    const double t = fma(-(double)v, steps.scale, base);
+    const uint32_t at = (uint32_t)t;  // (less than 0 and NaN: 0)
+    const uint32_t b = at < BINS - 1 ? at : spare;
+    if (COUNT) atomicAdd(&g.count[b], 1u);
+    if (WEIGH) {
+      const double r = __builtin_amdgcn_fract(t);
+      double e = fma(r, c4, c3);
+      e = fma(e, r, c2);
+      e = fma(e, r, c1);
+      e = fma(e, r, c0);
+      atomicAdd(&g.weight[b], (unsigned long long)__double_as_longlong(e) & 0xfffffffffffffull);
     }
-    return in || (upper < 0x7ff00001u && !(WEIGH && far));
   };
-  auto slow = [&](float v) {
+  auto below = [&](float v) {  // where the last step can still weigh: its categories
     const double t = steps.at(v);
-    if (!(t >= 0)) {
-      seen |= v != v ? 1 : 2;
-    } else if (WEIGH && t >= LOW && v > -INFINITY) {
-      const double e = exp_neg(fmax((LOW - t) * steps.width, -1000.0));
-      atomicAdd(&g.tail, (unsigned long long)__double_as_longlong(fma(e, one, 4503599627370496.0)) & 0xfffffffffffffull);
-    }
+    if (!(t >= (double)(BINS - 1)) || v == -INFINITY) return;
+    const double e = exp_neg(fmax(((double)(BINS - 1) - t) * steps.width, -1000.0));
+    atomicAdd(&g.tail, (unsigned long long)__double_as_longlong(fma(e, one, 4503599627370496.0)) & 0xfffffffffffffull);
   };
   src.template vectors<NT, 2>(
       [&](int c, const float* v) {
-        bool done = true;
+        float least = v[0];
 #pragma unroll
         for (int i = 0; i < S::N; i++) {
-          done &= fast(v[i]);
+          weigh(v[i]);
+          if (WEIGH) least = fminf(least, v[i]);
           __builtin_amdgcn_sched_barrier(0);  // one after the other: several at once spill registers
         }
-        if (!done)
+        if (far && steps.at(least) >= (double)(BINS - 1))
 #pragma unroll 1
-          for (int i = 0; i < S::N; i++) slow(src(c + i));
+          for (int i = 0; i < S::N; i++) below(src(c + i));
       },
       [&](int, float v) {
-        if (!fast(v)) slow(v);
+        weigh(v);
+        if (far) below(v);
       });
 }
 
@@ -1064,7 +1060,6 @@ __global__ __launch_bounds__(NT, 4) void sample_long(const T* logits, int64_t st
     top = -INFINITY;
     int categories = 0;
     if (!(first > -INFINITY && first < INFINITY)) {  // nothing to start from, or nothing but infinity counts
-      seen = 2;
       for (int c = threadIdx.x; c < cols; c += NT) {
         const float v = src(c);
         seen |= v != v;
@@ -1094,8 +1089,8 @@ __global__ __launch_bounds__(NT, 4) void sample_long(const T* logits, int64_t st
     top = block_max<NT>(top, g.fbuf[0]);  // (a barrier)
     if (threadIdx.x == 0) g.top = top;
     seen = uniform(g.seen);
-    if ((seen & 1) || top == -INFINITY) break;
-    if (seen) {
+    if (seen || top == -INFINITY) break;
+    if (!(first > -INFINITY && first < INFINITY) || steps.at(top) < 0) {
       // again from the row's largest logit; rows of infinities are left to the digits
       if (turn == 0 && top < INFINITY) {
         least = fminf(least, top);
