@@ -140,6 +140,45 @@ def test_sample_long_rows(cols, kind):
         cases.check_sample(z, u, mask=(torch.rand(4, cols, generator=g) < 0.5).to(DEV), top_p=0.8)
 
 
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("rows,cols", [(5, 2500), (5, 9001), (1100, 5001), (4, 70003)])
+def test_sample_rows_that_long_rows_kernels_treat_apart(rows, cols, kind):
+    """where the first vectors of a row say little or the wrong thing about it: the largest logits at its end, nothing open at
+    its start, few categories open at all, logits wider or closer than a step, one value throughout, infinities"""
+    g = torch.Generator().manual_seed(cols)
+    some = [0, rows // 2, rows - 1]
+
+    def check(z, mask=None, settings=(dict(), dict(top_p=0.9), dict(top_k=30, top_p=0.8), dict(min_p=0.1), dict(top_k=3000, top_p=0.99, min_p=1e-5))):
+        z, u = z.to(cases.DTYPES[kind]).to(DEV), torch.rand(rows, generator=g).to(DEV)
+        mask = None if mask is None else mask.to(DEV)
+        for s in settings:
+            got = ops.sample_logits(z, u, mask=mask, **s)
+            few = cases.check_sample(z[some], u[some], mask=None if mask is None else mask[some], **s)
+            assert torch.equal(got[some], few)
+
+    normal = torch.randn(rows, cols, generator=g)
+    late = normal.clone()
+    late[:, -7:] += 25
+    check(late)
+    late[:, -1] += 300
+    check(late)
+    bars = torch.ones(rows, cols, dtype=torch.bool)
+    bars[:, : cols - 900] = False
+    check(normal * 2, bars)  # nothing open where the steps begin
+    check(normal * 2, torch.rand(rows, cols, generator=g) < 12 / cols)  # a handful of categories open
+    one = torch.zeros(rows, cols, dtype=torch.bool)
+    one[:, cols - 3] = True
+    check(normal, one)
+    check(normal * 60, settings=(dict(), dict(top_k=50, temperature=0.7), dict(top_k=2000), dict(temperature=1e-6)))
+    check(normal * 1e-4, settings=(dict(), dict(top_p=0.5), dict(temperature=1e-4), dict(temperature=float("inf"), top_p=0.9)))
+    check(normal * 1e-3 + 900)
+    check(torch.full((rows, cols), -3.0))
+    infinite = normal.clone()
+    infinite[:, cols // 2] = float("inf")
+    infinite[:, 5] = -float("inf")
+    check(infinite)
+
+
 def edge_rows():
     inf, nan, low = float("inf"), float("nan"), torch.finfo(torch.float32).min
     z = torch.tensor([[1, 2, 3, 4], [-inf, -inf, -inf, -inf], [nan, inf, 0, 1], [nan, 1, 2, 3], [low, low, low, low],
