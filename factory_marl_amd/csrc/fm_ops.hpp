@@ -9,7 +9,8 @@
 namespace fm {
 int report(int code, const char* msg) noexcept;  // fm_api.hip: sets fm_last_error's text, returns code
 
-inline int type_size(int t) { return t == FM_DTYPE_F64 || t == FM_DTYPE_I64 ? 8 : t == FM_DTYPE_F32 || t == FM_DTYPE_I32 ? 4 : 2; }
+inline int type_size(int t) { return t == FM_DTYPE_F64 || t == FM_DTYPE_I64 ? 8 : t == FM_DTYPE_F32 || t == FM_DTYPE_I32
+    ? 4 : 2; }
 inline bool is_float_type(int t) { return t == FM_DTYPE_F32 || t == FM_DTYPE_F16 || t == FM_DTYPE_BF16; }
 inline bool aligned(const void* p, int bytes) { return ((uintptr_t)p % (uintptr_t)bytes) == 0; }
 // rows x cols elements and every row offset stay below 2^60

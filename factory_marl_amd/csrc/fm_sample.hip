@@ -1,14 +1,18 @@
 // fm_sample.hip -- one category of each row of logits, drawn with a given uniform number (include/factorysim.h
 // fm_sample_logits).
 //
-// A row's categories are ranked by a 64-bit place: the logit's bits, mapped so that whole numbers compare as the logits
-// do, above the complement of the index (the lower index first among equals).  Every setting keeps a leading part of
-// that ranking, and so does the share u of the kept weight, so all of them are the same question: which category is
-// the one where a running sum (of ones, or of weights) passes a number.
+// A row's categories are ranked by a 64-bit place: the logit's bits, mapped so that whole numbers compare as the logits do,
+// above the complement of the index (the lower index first among equals).  Every setting keeps a leading part of that ranking,
+// and so does the share u of the kept weight, so all of them are the same question: which category is the one where a running
+// sum (of ones, or of weights) passes a number.
 //
-// Weights are exp((logit - largest) / T) in multiples of 2^-s of the largest's, as 64-bit integers: sums are exact,
-// so no result depends on the order in which a launch happens to add, and a border that lies 2^-45 of the row's
-// weight away is still told apart (fp32 sums over 10^5 categories lose 2^-20 and would draw another category).
+// Weights are exp((logit - largest) / T) in multiples of 2^-s of the largest's, as 64-bit integers: sums are exact, so no
+// result depends on the order in which a launch happens to add, and a border that lies 2^-45 of the row's weight away is still
+// told apart (fp32 sums over 10^5 categories lose 2^-20 and would draw another category).
+//
+// Measured on an MI355X: 16384 x 2 fp32 3.4 us, 16384 x 1000 72, 1 x 32768 18, 37 x 50021 with a mask 30, 256 x 131072 bf16,
+// top_p 0.9, 61, of which reading it once would take 13.  Short rows are bound by their launch, rows of hundreds by the
+// instructions of sorting out one row each, long ones by float64 instructions (17 a logit) and a second read.
 #include <type_traits>
 
 #include "fm_ops_dev.hpp"
@@ -54,11 +58,14 @@ __device__ __forceinline__ double uniform(double v) {
                                           (uint32_t)__builtin_amdgcn_readfirstlane((int)b)));
 }
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
-__device__ __forceinline__ float uniform(float v) { return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(v))); }
+__device__ __forceinline__ float uniform(float v) {
+  return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(v)));
+}
 template <typename V>
 __device__ __forceinline__ const GLOBAL V* uniform(const V* v) {
   const uint64_t b = (uint64_t)v;
-  return (const GLOBAL V*)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(b >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((int)b));
+  return (const GLOBAL V*)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(b >> 32))
+      << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((int)b));
 }
 __device__ __forceinline__ Row uniform(Row o) {
   o.inv_t = uniform(o.inv_t);
@@ -195,9 +202,10 @@ __device__ __forceinline__ uint64_t sort_lanes(uint64_t p, int j) {
 
 // ---------------------------------------------------------------------------------------------- up to 64 categories
 // G lanes a row, one category each: sorted by exchanging places between lanes, then every setting is a prefix of the
-// group's lanes.  Rows of two categories fill a wave 32 at a time.
+// group's lanes.  Rows of two categories fill a wave 32 at a time: 65536 of them take 5 us, of 33 categories 42.
 template <typename T, int G>
-__global__ __launch_bounds__(256) void sample_group(const T* logits, int64_t stride, const uint8_t* mask, int64_t mask_stride, Settings a, int64_t* out,
+__global__ __launch_bounds__(256) void sample_group(const T* logits, int64_t stride, const uint8_t* mask, int64_t mask_stride,
+    Settings a, int64_t* out,
                                                     int64_t rows, int cols) {
   const int lane = threadIdx.x & 63, j = lane & (G - 1), base = lane - j;
   const uint64_t group = (G == 64 ? ~0ull : (1ull << G) - 1) << base;
@@ -346,13 +354,14 @@ __device__ uint64_t draw_from(List<LN>& l, int n, const Row& o) {
 }
 
 // ---------------------------------------------------------------------------------------------- up to 2048 categories
-// A wave a row, R logits a lane in registers, no barriers.  Weights go to 256 steps of the logit in LDS; the step in which a sum
-// passes a number is found by the lanes' running sums, and its categories, at most 64 as a rule, are compared with each
-// other, one a lane.
+// A wave a row, R logits a lane in registers, no barriers.  Weights go to 256 steps of the logit in LDS; the step in which a
+// sum passes a number is found by the lanes' running sums, and its categories, at most 64 as a rule, are compared with each
+// other, one a lane.  16384 x 1000 takes 72 us, sorting the rows in LDS, a block each, 296.
 constexpr int WBINS = 256;
 
 __device__ __forceinline__ uint64_t read_lane(uint64_t v, int lane) {
-  return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)v, lane);
+  return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane)
+      << 32 | (uint32_t)__builtin_amdgcn_readlane((int)v, lane);
 }
 
 template <typename T, bool MASKED, int R>
@@ -404,7 +413,8 @@ struct WaveRow {
     wsum = read_lane(at_w, l);
     return __builtin_amdgcn_readlane(found, l);
   }
-  // The category at which the running sum (of ones, or of weights) passes `number`: its place, and the weight up to and with it.
+  // The category at which the running sum (of ones, or of weights) passes `number`: its place, and the weight up to and with
+  // it.
   __device__ __forceinline__ uint64_t find(bool by_count, uint64_t number, Lds& g, const Row& o, uint64_t& upto) const {
     uint64_t sum, wsum;
     const int step = find_step(by_count, number, sum, wsum);
@@ -467,7 +477,8 @@ struct WaveRow {
 };
 
 template <typename T, bool MASKED, int R>
-__global__ __launch_bounds__(256, R > 16 ? 2 : 4) void sample_wave(const T* logits, int64_t stride, const uint8_t* mask, int64_t mask_stride, Settings a, int64_t* out,
+__global__ __launch_bounds__(256, R > 16 ? 2 : 4) void sample_wave(const T* logits, int64_t stride, const uint8_t* mask,
+    int64_t mask_stride, Settings a, int64_t* out,
                                                                  int64_t rows, int cols) {
   typedef WaveRow<T, MASKED, R> W;
   constexpr int N = W::N;
@@ -478,7 +489,8 @@ __global__ __launch_bounds__(256, R > 16 ? 2 : 4) void sample_wave(const T* logi
   const Row o = uniform(row_settings(a, r));
   W w;
   w.lane = threadIdx.x & 63;
-  const Source<T, MASKED> src{(const GLOBAL T*)(logits + r * stride), (const GLOBAL uint8_t*)(MASKED ? mask + r * mask_stride : nullptr), cols};
+  const Source<T, MASKED> src{(const GLOBAL T*)(logits + r * stride),
+      (const GLOBAL uint8_t*)(MASKED ? mask + r * mask_stride : nullptr), cols};
 #pragma unroll
   for (int i = 0; i < W::V; i++) {  // whole vectors; the row's last elements one at a time
     const int c = (i * 64 + w.lane) * N;
@@ -520,7 +532,8 @@ __global__ __launch_bounds__(256, R > 16 ? 2 : 4) void sample_wave(const T* logi
       });
       found = read_lane(sort_lanes<64>(found, w.lane), 0);
     } else {
-      // steps down to weights of e^-32 (with a T of next to nothing, to what float32 can tell apart), or to the row's least logit
+      // steps down to weights of e^-32 (with a T of next to nothing, to what float32 can tell apart), or to the row's least
+      // logit
       const float range = w.top - least, reach = fminf(range, fmaxf((float)(32.0 / o.inv_t), range / 4096.0f));
       w.scale = uniform(reach > 0 ? fminf((float)WBINS / reach, 3e38f) : 0.0f);
       const bool counted = o.top_k > 0 && o.top_k < cols;
@@ -564,7 +577,8 @@ __global__ __launch_bounds__(256, R > 16 ? 2 : 4) void sample_wave(const T* logi
           sum = kept < sum ? kept : sum;
         }
         uint64_t upto;
-        found = w.find(stage == 0, stage == 0 ? (uint64_t)o.top_k - 1 : stage == 1 ? border_of(o.top_p, sum) : target_of(o.u, sum), g, o, upto);
+        found = w.find(stage == 0, stage == 0 ? (uint64_t)o.top_k - 1 : stage == 1 ? border_of(o.top_p, sum)
+            : target_of(o.u, sum), g, o, upto);
         sum = upto < sum ? upto : sum;
       }
     }
@@ -573,16 +587,18 @@ __global__ __launch_bounds__(256, R > 16 ? 2 : 4) void sample_wave(const T* logi
 }
 
 // ---------------------------------------------------------------------------------------------- longer rows
-// One block a row, two passes over it as a rule.  The first counts or weighs the categories by steps of their logit, the
-// second lists and sorts those of the few steps in which a border and the drawn category lie.
+// One block a row, two passes over it as a rule.  The first counts or weighs the categories by steps of their logit, the second
+// lists and sorts those of the few steps in which a border and the drawn category lie.
 //
-// Steps are `scale` to a logit, counted down from HEAD at the largest logit of the row's first vectors (one for each
-// thread), so that no pass is needed to find the row's own largest; should one lie above step 0, the pass is made again.
-// With t = (first - v) scale + HEAD, step b = floor(t) and r = t - b, a category weighs exp(-r width) times what the top of its step
-// does, width = 1 / (scale T) <= 0.022 (32 steps to a power of two; more where the first vectors are closer together).  A
-// polynomial of degree 4 in r gives that to 5e-13 (four operations, 15 with the step's), and only the steps' sums are scaled
-// by a proper exp.  An equal logit weighs exactly as much: scale has 16 bits, which makes first * scale + HEAD, and with it t
-// of the first logit, exact.
+// Steps are `scale` to a logit, counted down from HEAD at the largest logit of the row's first vectors (one for each thread),
+// so that no pass is needed to find the row's own largest; should one lie above step 0, the pass is made again. With t = (first
+// - v) scale + HEAD, step b = floor(t) and r = t - b, a category weighs exp(-r width) times what the top of its step does,
+// width = 1 / (scale T) <= 0.022 (32 steps to a power of two; more where the first vectors are closer together).  A polynomial
+// of degree 4 in r gives that to 5e-13 (four operations, 15 with the step's), and only the steps' sums are scaled by a proper
+// exp.  An equal logit weighs exactly as much: scale has 16 bits, which makes first * scale + HEAD, and with it t of the first
+// logit, exact.
+//
+// 256 rows of 131072 bf16, a CU each: first vectors 4 us, first pass 20, sums of steps 3, second pass and list 16, draw 4.
 constexpr int BINS = 2048, HEAD = 512, DIGIT = 11;
 
 struct Steps {
@@ -654,17 +670,20 @@ __device__ __forceinline__ uint64_t block_before(uint64_t mine, unsigned long lo
 // (which tells whether one lay above the steps: those went to step 0, and the pass is made again), the number of its
 // categories (COUNT), and in `seen` a NaN.  The last step's count is what the others leave, its weight is g.tail.
 template <int NT, bool COUNT, bool WEIGH, typename S>
-__device__ __forceinline__ void weigh_steps(const S& src, const Steps& steps, double one, Long<NT>& g, float& top, int& categories, int& seen) {
+__device__ __forceinline__ void weigh_steps(const S& src, const Steps& steps, double one, Long<NT>& g, float& top,
+    int& categories, int& seen) {
   const bool far = WEIGH && !steps.past();
   // exp(-r width) = 1 + r (c1 + r (c2 + r (c3 + r c4))), exact at r = 0: its series with the term of r^5 put into the lower
-  // ones by r^4 = 2 r^3 - 5/4 r^2 + r/4 - 1/128, which Chebyshev's polynomial of degree 4 on 0 .. 1 gives to 1/128; 5e-13 in all.
-  // In units of 2^-s, and with 2^52 added, which leaves the whole number in the low bits
+  // ones by r^4 = 2 r^3 - 5/4 r^2 + r/4 - 1/128, which Chebyshev's polynomial of degree 4 on 0 .. 1 gives to 1/128; 5e-13 in
+  // all. In units of 2^-s, and with 2^52 added, which leaves the whole number in the low bits
   const double w = steps.width, e5 = -w * w * w * w * w / 120;
-  const double c1 = uniform(one * (-w - e5 / 128)), c2 = uniform(one * (w * w / 2 + e5 / 4)), c4 = uniform(one * (w * w * w * w / 24 + e5 * 2));
+  const double c1 = uniform(one * (-w - e5 / 128)), c2 = uniform(one * (w * w / 2 + e5 / 4)),
+      c4 = uniform(one * (w * w * w * w / 24 + e5 * 2));
   // an operation takes one operand from scalar registers: the others stay in vector registers
   double c3 = one * (-w * w * w / 6 - e5 * 1.25), c0 = one + 4503599627370496.0, base = steps.base;
   asm volatile("" : "+v"(c3), "+v"(c0), "+v"(base));
-  const uint32_t spare = BINS + 1 + (threadIdx.x & 63);  // where the weight of what lies below the steps goes, each lane's its own
+  // where the weight of what lies below the steps goes, each lane's its own
+  const uint32_t spare = BINS + 1 + (threadIdx.x & 63);
   auto weigh = [&](float v) {
     top = fmaxf(top, v);
     seen |= v != v;
@@ -768,7 +787,8 @@ __device__ __forceinline__ void add(Long<NT>& f, int b, uint64_t w) {
   const int b0 = __builtin_amdgcn_readfirstlane(b);
   if (__all(b == b0)) {
     const uint64_t active = __ballot(1);
-    const uint64_t w0 = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(w >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((int)w);
+    const uint64_t w0 = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(w >> 32))
+        << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((int)w);
     if (__all(w == w0)) {
       if ((threadIdx.x & 63) == __ffsll((unsigned long long)active) - 1) {
         atomicAdd(&f.count[b0], (uint32_t)__popcll(active));
@@ -854,7 +874,8 @@ __device__ __noinline__ uint64_t draw_by_digits() {
   const Source<T, MASKED> src = shared_source<T, MASKED, NT>();
   const float top = uniform(f.top);
   const Row o = uniform(f.o);
-  uint64_t n = 0, all = 0, most = 0;  // categories, their weight, the weight of those that min_p keeps (a leading part, as every setting's)
+  // categories, their weight, the weight of those that min_p keeps (a leading part, as every setting's)
+  uint64_t n = 0, all = 0, most = 0;
   src.template each<NT>([&](int, float v) {
     const uint64_t w = v > -INFINITY ? weight_of(v, top, o) : 0;
     n += v > -INFINITY;
@@ -872,7 +893,8 @@ __device__ __noinline__ uint64_t draw_by_digits() {
     if (stage == 0 && (o.top_k <= 0 || (uint64_t)o.top_k >= n)) continue;
     if (stage == 1 && o.top_p >= 1) continue;
     if (stage == 2 && most < sum) sum = most;
-    find<NT>(stage == 0, src, top, o, stage == 0 ? (uint64_t)o.top_k - 1 : stage == 1 ? border_of(o.top_p, sum) : target_of(o.u, sum), f);
+    find<NT>(stage == 0, src, top, o, stage == 0 ? (uint64_t)o.top_k - 1 : stage == 1 ? border_of(o.top_p, sum)
+        : target_of(o.u, sum), f);
     if (stage == 2) return f.place;
     sum = f.upto;
     __syncthreads();
@@ -920,13 +942,15 @@ __device__ __forceinline__ uint64_t draw_by_steps(const Steps& steps, float top,
   const bool border = b1 >= 0;
   // the draw's step is known but for how much of the border's steps is kept
   int t0 = step_of(g, g.weight, target_of(o.u, border && g.weight[b0] ? (uint64_t)g.weight[b0] : border ? 1 : sum));
-  int t1 = border ? step_of(g, g.weight, target_of(o.u, (uint64_t)g.weight[b1 + 1] < sum ? (uint64_t)g.weight[b1 + 1] : sum)) : t0;
+  int t1 = border ? step_of(g, g.weight, target_of(o.u, (uint64_t)g.weight[b1 + 1] < sum ? (uint64_t)g.weight[b1 + 1] : sum))
+      : t0;
   for (int turn = 0; turn < 2; turn++) {
     // first both in one list, then, should they be too many, the border alone and the one step of the draw
     if (turn && !border) return 0;
     const bool together = turn == 0;
     const bool joined = together && border && b0 <= t1 + 1;  // one stretch of steps
-    if (together ? list_steps<T, MASKED, NT>(t0, border && t1 > b1 ? b1 : t1, b0, b1) : list_steps<T, MASKED, NT>(b0, b1, 0, -1)) {
+    if (together ? list_steps<T, MASKED, NT>(t0, border && t1 > b1 ? b1 : t1, b0, b1)
+        : list_steps<T, MASKED, NT>(b0, b1, 0, -1)) {
       int split = 0;  // where the border's steps begin
       uint64_t base = g.weight[border ? (joined ? (t0 < b0 ? t0 : b0) : b0) : t0];
       const uint64_t tbase = joined ? base : g.weight[t0];
@@ -973,12 +997,14 @@ __device__ __forceinline__ uint64_t draw_by_steps(const Steps& steps, float top,
 }
 
 template <typename T, bool MASKED, int NT>
-__global__ __launch_bounds__(NT, 4) void sample_long(const T* logits, int64_t stride, const uint8_t* mask, int64_t mask_stride, Settings a, int64_t* out,
+__global__ __launch_bounds__(NT, 4) void sample_long(const T* logits, int64_t stride, const uint8_t* mask, int64_t mask_stride,
+    Settings a, int64_t* out,
                                                   int64_t rows, int cols) {
   Long<NT>& g = shared<NT>();
   const int64_t r = blockIdx.x + (int64_t)gridDim.x * blockIdx.y;
   if (r >= rows) return;
-  const Source<T, MASKED> src{(const GLOBAL T*)(logits + r * stride), (const GLOBAL uint8_t*)(MASKED ? mask + r * mask_stride : nullptr), cols};
+  const Source<T, MASKED> src{(const GLOBAL T*)(logits + r * stride),
+      (const GLOBAL uint8_t*)(MASKED ? mask + r * mask_stride : nullptr), cols};
   const Row o = uniform(row_settings(a, r));
   float top = -INFINITY;
   int wrong = o.nan;
@@ -1039,8 +1065,9 @@ __global__ __launch_bounds__(NT, 4) void sample_long(const T* logits, int64_t st
   }
   const bool counted = o.top_k > 0 && o.top_k < cols, weighed = !counted || o.top_k > Long<NT>::LISTED / 2;
   for (int turn = 0; turn < 2; turn++) {
-    // a power of two of the weight in 32 steps; narrower where the first vectors (enough of them that are not barred) lie within 1024
-    // T counts as 2^-35 |first| at least: the next float32 below would still weigh e^-2048, and first * scale stays below 2^41
+    // a power of two of the weight in 32 steps; narrower where the first vectors (enough of them that are not barred) lie
+    // within 1024 T counts as 2^-35 |first| at least: the next float32 below would still weigh e^-2048, and first * scale stays
+    // below 2^41
     const double most = 34359738368.0 / fabs((double)first), inv_t = fmin(o.inv_t, most);
     const double close = open < 256 ? 0.0 : 1024.0 / ((double)first - (double)least);
     const double wanted = fmin(fmin(fmax(fmax(32.0 * 1.4426950408889634 * inv_t, close), 1e-30), 64.0 * most), 1e300);
@@ -1111,7 +1138,8 @@ __global__ __launch_bounds__(NT, 4) void sample_long(const T* logits, int64_t st
       uint64_t sum = 0;
       for (int i = 0; i < EACH; i++) {
         const uint64_t m = b0 + i < BINS - 1 ? g.weight[b0 + i] : g.tail;
-        const uint64_t w = m ? (uint64_t)rint((double)m * exp_neg(fmax((double)(HEAD - b0 - i) * steps.width - shift, -1000.0))) : 0;
+        const uint64_t w = m ? (uint64_t)rint((double)m * exp_neg(fmax((double)(HEAD - b0 - i) * steps.width - shift,
+            -1000.0))) : 0;
         g.weight[b0 + i] = sum;
         sum += w;
       }
@@ -1149,7 +1177,8 @@ int shift_of(int64_t cols) {  // the sum of cols weights of at most 2^s stays be
 // CU) where that fills the chip or the row has little for more, else of 1024.
 template <typename T, bool MASKED>
 void launch(const fm_sample_args& a) {
-  const Settings s{a.temperature, a.top_p, a.min_p, a.top_k, a.temperature_rows, a.top_p_rows, a.min_p_rows, a.top_k_rows, a.u, a.u_dtype == FM_DTYPE_F64, shift_of(a.cols)};
+  const Settings s{a.temperature, a.top_p, a.min_p, a.top_k, a.temperature_rows, a.top_p_rows, a.min_p_rows, a.top_k_rows, a.u,
+      a.u_dtype == FM_DTYPE_F64, shift_of(a.cols)};
   hipStream_t st = (hipStream_t)a.stream;
   const int cols = (int)a.cols;
   auto blocks = [&](int rows_each) {

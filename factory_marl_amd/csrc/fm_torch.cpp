@@ -1,5 +1,5 @@
-// fm_torch.cpp -- the differentiable operators as autograd nodes: factory_marl_amd/ops.py checks and shapes the arguments and calls
-// torch.ops.factorysim.*, whose backward passes run here without the interpreter (a Python node waits for it on the
+// fm_torch.cpp -- the differentiable operators as autograd nodes: factory_marl_amd/ops.py checks and shapes the arguments and
+// calls torch.ops.factorysim.*, whose backward passes run here without the interpreter (a Python node waits for it on the
 // engine's thread: a layer norm of 64 x 128, forward and backward, took 105 us of host time with one and takes 60 like this).
 // All computing is the library's; its entry points are handed over once, by `bind`.
 #include <ATen/ATen.h>
@@ -71,7 +71,8 @@ Tensor workspace(Args& a, int64_t bytes, const Tensor& like) {
 // a backward pass's results; differentiating them is refused, where a graph of them is being made
 variable_list once(variable_list out) {
   if (!at::GradMode::is_enabled()) return out;
-  auto refuse = std::make_shared<torch::autograd::DelayedError>("factorysim: this operator is differentiable once", (int)out.size());
+  auto refuse = std::make_shared<torch::autograd::DelayedError>("factorysim: this operator is differentiable once",
+      (int)out.size());
   return (*refuse)(std::move(out));
 }
 

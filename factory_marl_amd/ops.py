@@ -3,8 +3,8 @@ fm_distill.hip): layer norm, drawing categories from logits, distillation from a
 
 GPU tensors are computed on torch's current stream of their device, CPU tensors by the library's CPU backend (as
 ``FactoryVecEnv(device=-1)``); there is no other path, a missing library raises.  Inputs may have any leading shape and
-row stride; one whose last dimension is not adjacent in memory is copied first.  Nothing synchronises and no buffer is kept between
-calls, so each call, forward or backward, can be captured into a graph.  A backward pass that is captured needs leaves
+row stride; one whose last dimension is not adjacent in memory is copied first.  Nothing synchronises and no buffer is
+kept between calls, so each call, forward or backward, can be captured into a graph.  A backward pass that is captured needs leaves
 that no live eager graph holds: torch ties a leaf's gradient to the stream of the graph that first used it.
 """
 import ctypes as C
@@ -144,7 +144,8 @@ class LayerNorm(nn.Module):
 def _row_setting(name, value, rows, logits, dtype):
     """a setting of each row as a contiguous tensor of the library's type"""
     if value.dtype.is_floating_point != (dtype == torch.float32) or value.dtype in (torch.bool, torch.float64):
-        raise TypeError(f"{name} of each row is {'a float32' if dtype == torch.float32 else 'an integer'} tensor, not {value.dtype}")
+        raise TypeError(f"{name} of each row is {'a float32' if dtype == torch.float32 else 'an integer'} tensor, "
+                        f"not {value.dtype}")
     if value.numel() != rows or (value.dim() > 1 and value.shape != logits.shape[:-1]):
         raise ValueError(f"{name} has shape {tuple(value.shape)}, the logits' rows {tuple(logits.shape[:-1])}")
     if value.device != logits.device:
@@ -165,7 +166,8 @@ def sample_logits(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, mas
     Each setting is a number or a tensor with one number for each row (float32; ``top_k`` integer).  temperature <= 0
     gives the largest logit; top_k <= 0, top_p >= 1 and min_p <= 0 are off.  ``mask`` (bool, logits' shape or
     [categories]) bars categories where it is False, whatever their logit; a logit of -inf bars its category too.
-    -1 stands for a row with no category left, with NaN in a logit that is not barred, or with a NaN in u or a setting.  logits: float32,
+    -1 stands for a row with no category left, with NaN in a logit that is not barred,
+        or with a NaN in u or a setting.  logits: float32,
     float16 or bfloat16; u: float32 or float64, in [0, 1).  Weights below 2^-46 of the largest count as nothing."""
     _float_input("logits", logits)
     if not torch.is_tensor(u) or u.dtype not in (torch.float32, torch.float64):

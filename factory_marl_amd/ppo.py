@@ -63,8 +63,8 @@ class ActorCriticPolicy(nn.Module):
     """SB3 ActorCriticPolicy with the default MlpExtractor (stable_baselines3/common/policies.py).
 
     layer_norm: ``ops.LayerNorm`` before every hidden tanh (SB3's checkpoints have none).  fused_sampling
-    (MultiDiscrete): actions are drawn by ``ops.sample_logits`` from one uniform number each, all dimensions of equal size in one
-    launch -- the same distribution as the default draws, from another use of the random stream."""
+    (MultiDiscrete): actions are drawn by ``ops.sample_logits`` from one uniform number each, all dimensions of equal size
+    in one launch -- the same distribution as the default draws, from another use of the random stream."""
 
     def __init__(self, obs_dim, action_dim=None, nvec=None, net_arch=(64, 64), log_std_init=0.0, ortho_init=True,
                  layer_norm=False, fused_sampling=False):

@@ -223,12 +223,14 @@ int fm_scene_mjcf(int num_arms, int max_num_objects, uint64_t seed, const char* 
  * Policy-head operators: layer norm, drawing categories from logits, distillation from a teacher's top logits.
  * They need no handle.  Conventions:
  *  - `device` is a GPU ordinal (buffers are device pointers, the work is queued on `stream`, a hipStream_t of that
- *    device or NULL for its default stream; the caller's current device is left as it was) or -1, the CPU backend (host pointers, done on return).
+ *    device or NULL for its default stream; the caller's current device is left as it was) or -1, the CPU backend (host pointers, done on
+ *    return).
  *  - Rows: `*_stride` is the distance of consecutive rows in elements (>= 0; 0 = every row the same), elements of one
  *    row are adjacent.  Outputs are contiguous.  No alignment beyond the element's own is needed.
  *  - Nothing is allocated, synchronised or kept between calls, so every call can be captured into a graph; the
  *    workspace (fm_*_workspace bytes, 16-byte aligned, contents ignored) belongs to one call at a time.
- *  - rows = 0 is valid and does nothing but zero a sum over rows.  Arguments are checked before anything runs: FM_EINVAL, no output touched. */
+ *  - rows = 0 is valid and does nothing but zero a sum over rows.  Arguments are checked before anything runs:
+ *    FM_EINVAL, no output touched. */
 #define FM_DTYPE_F32 0
 #define FM_DTYPE_F16 1
 #define FM_DTYPE_BF16 2
@@ -237,7 +239,8 @@ int fm_scene_mjcf(int num_arms, int max_num_objects, uint64_t seed, const char* 
 #define FM_DTYPE_I64 5
 
 /* y = (x - mean) * rstd * weight + bias over the last dimension, rstd = 1 / sqrt(variance + eps), biased variance;
- * statistics and sums in 32 bits.  x, y, dy, dx are of x_dtype; weight, bias and their gradients of param_dtype (x_dtype or F32). */
+ * statistics and sums in 32 bits.  x, y, dy, dx are of x_dtype; weight, bias and their gradients of param_dtype
+ * (x_dtype or F32). */
 typedef struct fm_layer_norm_args {
   int32_t device, x_dtype, param_dtype, reserved;
   int64_t rows, cols; /* cols >= 1 */
@@ -265,13 +268,15 @@ int64_t fm_layer_norm_workspace(int64_t rows, int64_t cols);
 
 /* Draws one category of each row: the row's categories are ranked by logit, the lower index first among equals, and
  * weigh w = exp((logit - largest) / temperature).  Kept are the first top_k, of those the shortest leading part that
- * holds at least top_p of their weight (the product as a double), of those the ones with w >= min_p; out is the first of the kept ones up to
- * which more than u of their weight lies.  mask (bytes, 0 = barred; any value may stand in a barred logit) and logits
+ * holds at least top_p of their weight (the product as a double), of those the ones with w >= min_p; out is the first of
+ * the kept ones up to which more than u of their weight lies.  mask (bytes, 0 = barred; any value may stand in a barred logit) and logits
  * of -inf bar a category; +inf outweighs everything finite.  A row with nothing left, with NaN in a logit that is not
- * barred or with a NaN setting gives -1.  Each setting is one number for all rows, or, where *_rows is not NULL, a float (top_k: int32) of each row's own.
+ * barred or with a NaN setting gives -1.  Each setting is one number for all rows, or, where *_rows is not NULL, a float
+ * (top_k: int32) of each row's own.
  * temperature <= 0: the largest logit; top_k <= 0, top_p >= 1, min_p <= 0: off; top_p <= 0 and min_p >= 1 keep the
- * largest (min_p: and its equals); u is meant to be in [0, 1) and is cut to what is kept.  Weights are summed as 64-bit integers
- * of 2^-45 or finer: results do not depend on the order of the sums. */
+ * largest (min_p: and its equals); u is meant to be in [0, 1) and is cut to what is kept.  Weights are whole multiples of
+ * 2^-s of the largest's, s = 51 or what 62 bits leave for the sum of cols of them (45 for 2^17 categories); what weighs
+ * less than half of that is never drawn.  Their sums are exact and do not depend on the order. */
 typedef struct fm_sample_args {
   int32_t device, dtype, u_dtype, reserved; /* u_dtype: F32 or F64 */
   int64_t rows, cols;                       /* 1 <= cols < 2^31 */
@@ -296,8 +301,8 @@ int64_t fm_sample_workspace(int64_t rows, int64_t cols);
 
 /* loss[i] = T^2 * sum over the listed entries of p (log p - log q[index]), q = softmax(logits / T) over all columns,
  * p = softmax(teacher / T) over the row's listed entries.  An entry with a negative index or a teacher logit of -inf
- * is not listed; a row without entries has loss 0 and gradient 0; an index >= cols makes the row's loss and gradient NaN; the same
- * index listed twice counts twice.  Backward: dlogits = grad[i] * T * (q - p at the listed places). */
+ * is not listed; a row without entries has loss 0 and gradient 0; an index >= cols makes the row's loss and
+ * gradient NaN; the same index listed twice counts twice.  Backward: dlogits = grad[i] * T * (q - p at the listed places). */
 typedef struct fm_distill_args {
   int32_t device, dtype, index_dtype, teacher_dtype; /* index_dtype: I32 or I64; teacher: F32, F16 or BF16 */
   int64_t rows, cols, k;                             /* 1 <= cols < 2^31, 1 <= k <= FM_DISTILL_MAX_K */
@@ -309,7 +314,8 @@ typedef struct fm_distill_args {
   int64_t teacher_stride;
   double temperature; /* > 0 */
   float* loss;        /* forward: [rows] */
-  float* stats;       /* [rows, 2], largest logit and sum of exp: written by the forward call (NULL: not kept), read by the backward call */
+  float* stats;       /* [rows, 2], largest logit and sum of exp: written by the forward call (NULL: not kept), read
+                         * by the backward call */
   const float* grad;  /* backward: [rows] with grad_stride */
   int64_t grad_stride;
   void* dlogits; /* backward: [rows, cols] */
