@@ -80,7 +80,7 @@ int check_norm(const fm_layer_norm_args* a, bool backward) {
   if (a->param_dtype != a->x_dtype && a->param_dtype != FM_DTYPE_F32) return bad("layer norm: param_dtype is x_dtype or F32");
   if (a->rows < 0 || a->cols < 1) return bad("layer norm: rows >= 0 and cols >= 1 are needed");
   if (a->x_stride < 0 || (backward && a->dy_stride < 0)) return bad("layer norm: negative row stride");
-  if (!fits(a->rows, a->cols, a->x_stride) || (backward && !fits(a->rows, a->cols, a->dy_stride)) || a->cols >= INT32_MAX)
+  if (!fits(a->rows, a->cols, a->x_stride) || (backward && !fits(a->rows, a->cols, a->dy_stride)) || a->cols > FM_MAX_COLS)
     return bad("layer norm: too many elements");
   const int xs = type_size(a->x_dtype), ps = type_size(a->param_dtype);
   if (!aligned(a->x, xs) || !aligned(a->weight, ps)) return bad("layer norm: misaligned pointer");
@@ -108,14 +108,14 @@ int check_sample(const fm_sample_args* a) {
   if (a->device < -1) return bad("sample: device is a GPU ordinal or -1");
   if (!is_float_type(a->dtype)) return bad("sample: dtype is F32, F16 or BF16");
   if (a->u_dtype != FM_DTYPE_F32 && a->u_dtype != FM_DTYPE_F64) return bad("sample: u_dtype is F32 or F64");
-  if (a->rows < 0 || a->cols < 1 || a->cols >= INT32_MAX) return bad("sample: rows >= 0 and 1 <= cols < 2^31 - 1 are needed");
+  if (a->rows < 0 || a->cols < 1 || a->cols > FM_MAX_COLS) return bad("sample: rows >= 0 and 1 <= cols <= 2^28 are needed");
   if (a->stride < 0 || a->mask_stride < 0) return bad("sample: negative row stride");
-  if (!fits(a->rows, a->cols, a->stride) || !fits(a->rows, a->cols, a->mask_stride) ||
-      a->rows >> 35) return bad("sample: too many elements");
+  if (!fits(a->rows, a->cols, a->stride) || !fits(a->rows, a->cols, a->mask_stride) || a->rows >> 35)
+    return bad("sample: too many elements");
   if (a->rows > 0 && (!a->logits || !a->u || !a->out)) return bad("sample: logits, u and out are needed");
   if (!aligned(a->logits, type_size(a->dtype)) || !aligned(a->u, type_size(a->u_dtype)) || !aligned(a->out, 8) ||
       !aligned(a->temperature_rows, 4) || !aligned(a->top_p_rows, 4) || !aligned(a->min_p_rows, 4) ||
-          !aligned(a->top_k_rows, 4))
+      !aligned(a->top_k_rows, 4))
     return bad("sample: misaligned pointer");
   if ((!a->temperature_rows && std::isnan(a->temperature)) || (!a->top_p_rows && std::isnan(a->top_p)) ||
       (!a->min_p_rows && std::isnan(a->min_p)))
@@ -129,9 +129,10 @@ int check_sample(const fm_sample_args* a) {
 int check_distill(const fm_distill_args* a, bool backward) {
   if (!a) return bad("distill: null argument");
   if (a->device < -1) return bad("distill: device is a GPU ordinal or -1");
-  if (!is_float_type(a->dtype) || !is_float_type(a->teacher_dtype)) return bad("distill: dtype and teacher_dtype are F32, F16 or BF16");
+  if (!is_float_type(a->dtype) || !is_float_type(a->teacher_dtype))
+    return bad("distill: dtype and teacher_dtype are F32, F16 or BF16");
   if (a->index_dtype != FM_DTYPE_I32 && a->index_dtype != FM_DTYPE_I64) return bad("distill: index_dtype is I32 or I64");
-  if (a->rows < 0 || a->cols < 1 || a->cols >= INT32_MAX) return bad("distill: rows >= 0 and 1 <= cols < 2^31 - 1 are needed");
+  if (a->rows < 0 || a->cols < 1 || a->cols > FM_MAX_COLS) return bad("distill: rows >= 0 and 1 <= cols <= 2^28 are needed");
   if (a->k < 1 || a->k > FM_DISTILL_MAX_K) return bad("distill: 1 <= k <= 1024 is needed");
   if (a->stride < 0 || a->index_stride < 0 || a->teacher_stride < 0 || (backward && a->grad_stride < 0))
     return bad("distill: negative row stride");
@@ -139,12 +140,12 @@ int check_distill(const fm_distill_args* a, bool backward) {
       (backward && !fits(a->rows, 1, a->grad_stride)))
     return bad("distill: too many elements");
   if (a->rows >> 35) return bad("distill: too many rows");
-  if (!(a->temperature > 0) || !(a->temperature >= 1e-30 &&
-      a->temperature <= 1e30)) return bad("distill: temperature is positive and within 1e-30 .. 1e30");
+  if (!(a->temperature >= 1e-30 && a->temperature <= 1e30))
+    return bad("distill: temperature is positive and within 1e-30 .. 1e30");
   if (a->rows > 0 && (!a->logits || !a->index || !a->teacher)) return bad("distill: logits, index and teacher are needed");
   if (a->rows > 0 && !backward && !a->loss) return bad("distill: loss is NULL");
-  if (a->rows > 0 && backward && (!a->stats || !a->grad ||
-      !a->dlogits)) return bad("distill: stats, grad and dlogits are needed");
+  if (a->rows > 0 && backward && (!a->stats || !a->grad || !a->dlogits))
+    return bad("distill: stats, grad and dlogits are needed");
   if (!aligned(a->logits, type_size(a->dtype)) || !aligned(a->index, type_size(a->index_dtype)) ||
       !aligned(a->teacher, type_size(a->teacher_dtype)) || !aligned(a->stats, 4) || !aligned(a->loss, 4) ||
       (backward && (!aligned(a->grad, 4) || !aligned(a->dlogits, type_size(a->dtype)))))

@@ -1,5 +1,5 @@
-// fm_torch.cpp -- the differentiable operators as autograd nodes: factory_marl_amd/ops.py checks and shapes the arguments and
-// calls torch.ops.factorysim.*, whose backward passes run here without the interpreter (a Python node waits for it on the
+// fm_torch.cpp -- the operators' calls from tensors: factory_marl_amd/ops.py checks and shapes the arguments and calls
+// torch.ops.factorysim.*, whose backward passes run here without the interpreter (a Python node waits for it on the
 // engine's thread: a layer norm of 64 x 128, forward and backward, took 105 us of host time with one and takes 60 like this).
 // All computing is the library's; its entry points are handed over once, by `bind`.
 #include <ATen/ATen.h>
@@ -24,6 +24,8 @@ struct Entries {
   decltype(&fm_distill_forward) distill_forward;
   decltype(&fm_distill_backward) distill_backward;
   decltype(&fm_distill_workspace) distill_workspace;
+  decltype(&fm_sample_logits) sample_logits;
+  decltype(&fm_sample_workspace) sample_workspace;
   decltype(&fm_last_error) last_error;
 } fm;
 
@@ -76,6 +78,12 @@ variable_list once(variable_list out) {
   return (*refuse)(std::move(out));
 }
 
+// a forward-mode derivative would be lost without a word
+void no_tangent(const Tensor& t) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t._fw_grad(0).defined(),
+                              "factorysim: this operator has no forward-mode derivative");
+}
+
 // ------------------------------------------------------------------ layer norm
 struct LayerNormBackward : public torch::autograd::Node {
   SavedVariable x, weight, stats;
@@ -123,6 +131,7 @@ struct LayerNormBackward : public torch::autograd::Node {
 Tensor layer_norm(const Tensor& x, const std::optional<Tensor>& weight, const std::optional<Tensor>& bias, double eps) {
   const Tensor w = weight.value_or(Tensor()), b = bias.value_or(Tensor());
   const bool graph = torch::autograd::compute_requires_grad(x, w, b);
+  no_tangent(x), no_tangent(w), no_tangent(b);
   const int64_t n = x.size(0);
   Tensor y = at::empty({n, x.size(1)}, x.options().requires_grad(false)), stats;
   fm_layer_norm_args a = {};
@@ -205,6 +214,7 @@ struct DistillBackward : public torch::autograd::Node {
 // z [rows, cols], index and teacher [rows, k], all with adjacent columns
 Tensor distill_loss(const Tensor& z, const Tensor& index, const Tensor& teacher, double temperature) {
   const bool graph = torch::autograd::compute_requires_grad(z);
+  no_tangent(z), no_tangent(teacher);
   fm_distill_args a = distill_args(z, index, teacher, temperature);
   const auto floats = z.options().dtype(at::kFloat).requires_grad(false);
   Tensor loss = at::empty({a.rows}, floats), stats;
@@ -224,10 +234,45 @@ Tensor distill_loss(const Tensor& z, const Tensor& index, const Tensor& teacher,
   torch::autograd::set_history(loss, node);
   return loss;
 }
+// ------------------------------------------------------------------ drawing categories
+// z [rows, cols] and mask (rows or one row of them) with adjacent columns, u and the settings of each row [rows], contiguous
+Tensor sample_logits(const Tensor& z, const Tensor& u, const std::optional<Tensor>& mask, double temperature, int64_t top_k,
+                     double top_p, double min_p, const std::optional<Tensor>& temperature_rows,
+                     const std::optional<Tensor>& top_k_rows, const std::optional<Tensor>& top_p_rows,
+                     const std::optional<Tensor>& min_p_rows) {
+  fm_sample_args a = {};
+  place(a, z);
+  a.dtype = code(z);
+  a.u_dtype = u.scalar_type() == at::kDouble ? FM_DTYPE_F64 : FM_DTYPE_F32;
+  a.rows = z.size(0);
+  a.cols = z.size(1);
+  a.logits = data(z);
+  a.stride = row_stride(z);
+  if (mask) {
+    a.mask = (const uint8_t*)data(*mask);
+    a.mask_stride = row_stride(*mask);
+  }
+  a.u = data(u);
+  a.temperature = temperature;
+  a.top_k = top_k;
+  a.top_p = top_p;
+  a.min_p = min_p;
+  if (temperature_rows) a.temperature_rows = (const float*)data(*temperature_rows);
+  if (top_k_rows) a.top_k_rows = (const int32_t*)data(*top_k_rows);
+  if (top_p_rows) a.top_p_rows = (const float*)data(*top_p_rows);
+  if (min_p_rows) a.min_p_rows = (const float*)data(*min_p_rows);
+  const Tensor out = at::empty({a.rows}, z.options().dtype(at::kLong).requires_grad(false));
+  a.out = (int64_t*)data(out);
+  const Tensor work = workspace(a, fm.sample_workspace(a.rows, a.cols), z);
+  check(fm.sample_logits(&a));
+  return out;
+}
 }  // namespace
 
 TORCH_LIBRARY(factorysim, m) {
   m.def("bind(int[] addresses) -> ()", &bind);
   m.def("layer_norm(Tensor x, Tensor? weight, Tensor? bias, float eps) -> Tensor", &layer_norm);
   m.def("distill_loss(Tensor logits, Tensor teacher_index, Tensor teacher_logits, float temperature) -> Tensor", &distill_loss);
+  m.def("sample_logits(Tensor logits, Tensor u, Tensor? mask, float temperature, int top_k, float top_p, float min_p, "
+        "Tensor? temperature_rows, Tensor? top_k_rows, Tensor? top_p_rows, Tensor? min_p_rows) -> Tensor", &sample_logits);
 }

@@ -5,7 +5,8 @@ GPU tensors are computed on torch's current stream of their device, CPU tensors 
 ``FactoryVecEnv(device=-1)``); there is no other path, a missing library raises.  Inputs may have any leading shape and
 row stride; one whose last dimension is not adjacent in memory is copied first.  Nothing synchronises and no buffer is
 kept between calls, so each call, forward or backward, can be captured into a graph.  A backward pass that is captured needs leaves
-that no live eager graph holds: torch ties a leaf's gradient to the stream of the graph that first used it.
+that no live eager graph holds: torch ties a leaf's gradient to the stream of the graph that first used it.  A row has at
+most 2^28 elements.
 """
 import ctypes as C
 import math
@@ -29,7 +30,7 @@ _loaded = None
 
 
 def _library():
-    """the library, its differentiable operators registered with torch (csrc/fm_torch.cpp)"""
+    """the library, its operators registered with torch (csrc/fm_torch.cpp)"""
     global _loaded
     if _loaded is None:
         L = _lib.load()
@@ -39,7 +40,7 @@ def _library():
             raise _lib.FactorySimError(f"{_NODES} not built: run `python __graft_entry__.py build`")
         torch.ops.load_library(_NODES)
         names = ("fm_layer_norm_forward", "fm_layer_norm_backward", "fm_layer_norm_workspace", "fm_distill_forward",
-                 "fm_distill_backward", "fm_distill_workspace", "fm_last_error")
+                 "fm_distill_backward", "fm_distill_workspace", "fm_sample_logits", "fm_sample_workspace", "fm_last_error")
         torch.ops.factorysim.bind([C.cast(getattr(L, n), C.c_void_p).value for n in names])
         _loaded = L
     return _loaded
@@ -54,24 +55,12 @@ def _call(op, *args):
         raise
 
 
-def _where(t):
-    """(device ordinal or -1, stream) of a tensor's calls"""
-    if t.is_cuda:
-        d = t.device.index
-        return d, torch._C._cuda_getCurrentRawStream(d)
-    return -1, None
-
-
 def _rows(t):
     """t as [rows, cols] with adjacent columns: a view where there is one"""
     if t.dim() != 2:
         n = t.shape[-1]
         t = t.reshape(-1 if n else 0, n)
     return t if t.shape[1] <= 1 or t.stride(1) == 1 else t.contiguous()
-
-
-def _stride(t):
-    return t.stride(0) if t.shape[0] > 1 else 0
 
 
 def _float_input(name, t):
@@ -91,10 +80,6 @@ def _same_device(t, **others):
             raise ValueError(f"{name} is on {o.device}, the first input on {t.device}")
 
 
-def _ptr(t):
-    return None if t is None else t.data_ptr()
-
-
 # ------------------------------------------------------------------ layer norm
 def layer_norm(x, weight=None, bias=None, eps=1e-5):
     """(x - mean) / sqrt(variance + eps) * weight + bias over the last dimension (biased variance), in x's dtype.
@@ -107,6 +92,8 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
     for name, p in (("weight", weight), ("bias", bias)):
         if p is None:
             continue
+        if not torch.is_tensor(p):
+            raise TypeError(f"{name} is a tensor or None")
         if p.dtype != x.dtype and p.dtype != torch.float32:
             raise TypeError(f"{name} is float32 or of x's dtype {x.dtype}, not {p.dtype}")
         if tuple(p.shape) != (v,):
@@ -166,9 +153,9 @@ def sample_logits(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, mas
     Each setting is a number or a tensor with one number for each row (float32; ``top_k`` integer).  temperature <= 0
     gives the largest logit; top_k <= 0, top_p >= 1 and min_p <= 0 are off.  ``mask`` (bool, logits' shape or
     [categories]) bars categories where it is False, whatever their logit; a logit of -inf bars its category too.
-    -1 stands for a row with no category left, with NaN in a logit that is not barred,
-        or with a NaN in u or a setting.  logits: float32,
-    float16 or bfloat16; u: float32 or float64, in [0, 1).  Weights below 2^-46 of the largest count as nothing."""
+    -1 stands for a row with no category left, with NaN in a logit that is not barred, or with a NaN in u or a setting.
+    logits: float32, float16 or bfloat16; u: float32 or float64, in [0, 1).  Weights below 2^-46 of the largest count as
+    nothing (2^-45 beyond 2^17 categories, and a bit less for each doubling)."""
     _float_input("logits", logits)
     if not torch.is_tensor(u) or u.dtype not in (torch.float32, torch.float64):
         raise TypeError("u is a float32 or float64 tensor")
@@ -176,12 +163,12 @@ def sample_logits(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, mas
         raise ValueError(f"u has shape {tuple(u.shape)}, the logits' rows {tuple(logits.shape[:-1])}")
     if u.device != logits.device:
         raise ValueError(f"u is on {u.device}, the logits on {logits.device}")
-    z = _rows(logits.detach())
+    z = _rows(logits)
     n, v = z.shape
     m = None
     if mask is not None:
-        if mask.dtype != torch.bool:
-            raise TypeError(f"mask is a bool tensor, not {mask.dtype}")
+        if not torch.is_tensor(mask) or mask.dtype != torch.bool:
+            raise TypeError(f"mask is a bool tensor, not {getattr(mask, 'dtype', type(mask))}")
         if mask.shape != logits.shape and tuple(mask.shape) != (v,):
             raise ValueError(f"mask has shape {tuple(mask.shape)}, the logits {tuple(logits.shape)}")
         if mask.device != logits.device:
@@ -199,18 +186,10 @@ def sample_logits(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, mas
     t, p, q, k = float(temperature), float(top_p), float(min_p), int(top_k)
     if t != t or p != p or q != q:
         raise ValueError("temperature, top_p and min_p are numbers, not NaN")
-    u = u.detach().reshape(-1).contiguous() if u.dim() != 1 or not u.is_contiguous() else u
-    L = _library()
-    dev, stream = _where(z)
-    out = torch.empty(logits.shape[:-1], dtype=torch.int64, device=z.device)
-    need = L.fm_sample_workspace(n, v) if dev >= 0 else 0
-    work = torch.empty(need, dtype=torch.uint8, device=z.device) if need else None
-    a = _lib.FmSampleArgs(dev, _DTYPES[z.dtype], _lib.FM_DTYPE_F32 if u.dtype == torch.float32 else _lib.FM_DTYPE_F64, 0,
-                          n, v, z.data_ptr(), _stride(z), _ptr(m), 0 if m is None else _stride(m), u.data_ptr(), t, p,
-                          q, min(max(k, 0), 2**31 - 1), _ptr(t_rows), _ptr(p_rows), _ptr(q_rows), _ptr(k_rows), out.data_ptr(),
-                          _ptr(work), need, stream)
-    _lib.check(L.fm_sample_logits(a), L)
-    return out
+    u = u.reshape(-1).contiguous() if u.dim() != 1 or not u.is_contiguous() else u
+    _library()
+    out = _call(torch.ops.factorysim.sample_logits, z, u, m, t, min(max(k, 0), 2**31 - 1), p, q, t_rows, k_rows, p_rows, q_rows)
+    return out if logits.dim() == 2 else out.view(logits.shape[:-1])
 
 
 # ------------------------------------------------------------------ distillation

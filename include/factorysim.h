@@ -231,6 +231,7 @@ int fm_scene_mjcf(int num_arms, int max_num_objects, uint64_t seed, const char* 
  *    workspace (fm_*_workspace bytes, 16-byte aligned, contents ignored) belongs to one call at a time.
  *  - rows = 0 is valid and does nothing but zero a sum over rows.  Arguments are checked before anything runs:
  *    FM_EINVAL, no output touched. */
+#define FM_MAX_COLS (1 << 28) /* the most elements of a row: kernels count them, twice over and a block more, in 32 bits */
 #define FM_DTYPE_F32 0
 #define FM_DTYPE_F16 1
 #define FM_DTYPE_BF16 2
@@ -243,7 +244,7 @@ int fm_scene_mjcf(int num_arms, int max_num_objects, uint64_t seed, const char* 
  * (x_dtype or F32). */
 typedef struct fm_layer_norm_args {
   int32_t device, x_dtype, param_dtype, reserved;
-  int64_t rows, cols; /* cols >= 1 */
+  int64_t rows, cols; /* 1 <= cols <= FM_MAX_COLS */
   const void* x;
   int64_t x_stride;
   const void* weight; /* [cols]; NULL = ones */
@@ -279,7 +280,7 @@ int64_t fm_layer_norm_workspace(int64_t rows, int64_t cols);
  * less than half of that is never drawn.  Their sums are exact and do not depend on the order. */
 typedef struct fm_sample_args {
   int32_t device, dtype, u_dtype, reserved; /* u_dtype: F32 or F64 */
-  int64_t rows, cols;                       /* 1 <= cols < 2^31 */
+  int64_t rows, cols;                       /* 1 <= cols <= FM_MAX_COLS */
   const void* logits;
   int64_t stride;
   const uint8_t* mask; /* [rows, cols] with mask_stride; NULL = none */
@@ -305,7 +306,7 @@ int64_t fm_sample_workspace(int64_t rows, int64_t cols);
  * gradient NaN; the same index listed twice counts twice.  Backward: dlogits = grad[i] * T * (q - p at the listed places). */
 typedef struct fm_distill_args {
   int32_t device, dtype, index_dtype, teacher_dtype; /* index_dtype: I32 or I64; teacher: F32, F16 or BF16 */
-  int64_t rows, cols, k;                             /* 1 <= cols < 2^31, 1 <= k <= FM_DISTILL_MAX_K */
+  int64_t rows, cols, k;                             /* 1 <= cols <= FM_MAX_COLS, 1 <= k <= FM_DISTILL_MAX_K */
   const void* logits;
   int64_t stride;
   const void* index; /* [rows, k] */

@@ -397,6 +397,27 @@ def test_two_streams_at_once():
         assert all(torch.equal(a, b) for a, b in zip(out, want[i]))
 
 
+def test_more_rows_than_blocks_in_a_line_of_the_grid():
+    """rows repeat a few kinds, whose results are those of a call with these few"""
+    g = torch.Generator().manual_seed(41)
+    for rows, cols in [(2**22 + 5, 64), (2**22 + 5, 65), (2**20 + 5, 2100)]:
+        z = (2 * torch.randn(1, cols, generator=g)).to(DEV, torch.bfloat16)
+        u, kind = torch.rand(1000, generator=g).to(DEV), torch.arange(rows, device=DEV) % 1000
+        few = ops.sample_logits(z.expand(1000, cols), u, top_p=0.95)
+        assert torch.equal(ops.sample_logits(z.expand(rows, cols), u[kind], top_p=0.95), few[kind])
+    for rows, cols, k in [(2**22 + 5, 33, 2), (2**20 + 5, 3, 65)]:
+        z, at = torch.randn(1000, cols, generator=g).to(DEV), torch.randint(cols, (1000, k), generator=g, dtype=torch.int32).to(DEV)
+        t, kind = torch.randn(1, k, generator=g).to(DEV), torch.arange(rows, device=DEV) % 1000
+
+        def run(z, at, t):
+            z = z.requires_grad_()
+            loss = ops.distill_loss(z, at, t, temperature=1.3)
+            return (loss, *torch.autograd.grad(loss.sum(), z))
+
+        few, all_rows = run(z, at, t.expand(1000, k)), run(z.detach()[kind], at[kind], t.expand(rows, k))
+        assert all(torch.equal(b, a[kind]) for a, b in zip(few, all_rows))
+
+
 def test_gpu_and_cpu_backends_agree():
     for rows, cols in ((40, 2), (9, 500), (3, 5000)):
         s = _state(rows, cols, 7)

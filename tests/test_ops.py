@@ -275,6 +275,36 @@ def test_c_refusals():
     assert (out == 7).all() and (tok == 7).all() and (loss == 7).all()
 
 
+def test_rows_beyond_the_most_columns_are_refused():
+    """2^28 columns are taken (no rows: nothing is read), one more is not"""
+    L = _lib.load()
+    norm, sample = _lib.FmLayerNormArgs(device=-1, cols=2**28), _lib.FmSampleArgs(device=-1)
+    distill = _lib.FmDistillArgs(device=-1, cols=2**28, k=1, index_dtype=_lib.FM_DTYPE_I32, temperature=1.0)
+    assert L.fm_layer_norm_forward(norm) == L.fm_distill_forward(distill) == 0
+    norm.cols = sample.cols = distill.cols = 2**28 + 1
+    assert L.fm_layer_norm_forward(norm) == L.fm_layer_norm_backward(norm) == L.fm_sample_logits(sample) == -1
+    assert L.fm_distill_forward(distill) == L.fm_distill_backward(distill) == -1
+
+
+def test_forward_mode_derivatives_are_refused():
+    ad = torch.autograd.forward_ad
+    x, z = torch.randn(3, 4), torch.randn(3, 5)
+    with ad.dual_level():
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            ops.layer_norm(ad.make_dual(x, torch.ones(3, 4)))
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            ops.layer_norm(x, ad.make_dual(torch.ones(4), torch.ones(4)))
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            ops.distill_loss(ad.make_dual(z, z), torch.zeros(3, 1, dtype=torch.int64), torch.zeros(3, 1))
+
+
+def test_arguments_that_are_no_tensors_are_refused():
+    with pytest.raises(TypeError):
+        ops.layer_norm(torch.randn(3, 4), [1.0] * 4)
+    with pytest.raises(TypeError):
+        ops.sample_logits(torch.randn(3, 4), torch.rand(3), mask=[True] * 4)
+
+
 def test_missing_device_is_an_error_and_not_the_cpu():
     if torch.cuda.is_available():
         pytest.skip("a GPU is present")
