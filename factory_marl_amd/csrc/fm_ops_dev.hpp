@@ -114,10 +114,7 @@ __device__ __forceinline__ V block_sum(V v, V* buf) {
   if (NT == 64) return v;
   if ((threadIdx.x & 63) == 0) buf[threadIdx.x >> 6] = v;
   __syncthreads();
-  V s = buf[0];
-#pragma unroll
-  for (int i = 1; i < NT / 64; i++) s += buf[i];
-  return s;
+  return group_sum<NT / 64>(buf[threadIdx.x % (NT / 64)]);
 }
 template <int NT>
 __device__ __forceinline__ float block_max(float v, float* buf) {
@@ -125,10 +122,7 @@ __device__ __forceinline__ float block_max(float v, float* buf) {
   if (NT == 64) return v;
   if ((threadIdx.x & 63) == 0) buf[threadIdx.x >> 6] = v;
   __syncthreads();
-  float s = buf[0];
-#pragma unroll
-  for (int i = 1; i < NT / 64; i++) s = fmaxf(s, buf[i]);
-  return s;
+  return group_max<NT / 64>(buf[threadIdx.x % (NT / 64)]);
 }
 
 // Makes `device` current for one call's launches and restores the caller's; status() reports what the launches did.

@@ -602,7 +602,7 @@ __global__ __launch_bounds__(256, R > 16 ? 2 : 4) void sample_wave(const T* logi
 constexpr int BINS = 2048, HEAD = 512, DIGIT = 11;
 
 struct Steps {
-  double first, scale, width;  // width: 1 / (scale T)
+  double first, scale, inv, width;  // inv: 1 / scale; width: 1 / (scale T)
   double base;                 // first * scale + HEAD
   __device__ __forceinline__ double at(float v) const { return fma(-(double)v, scale, base); }
   // never falls as v falls; -1 above the steps, the last step takes all that lies below
@@ -612,7 +612,7 @@ struct Steps {
   __device__ __forceinline__ bool past() const { return (BINS - 1 - HEAD) * width >= 33.0; }
   // all logits of steps b0 .. b1 (and a few others) lie within `half` of `mid`
   __device__ __forceinline__ void around(int b0, int b1, float& mid, float& half) const {
-    const double d0 = (double)(HEAD - b0) / scale, d1 = (double)(HEAD - b1 - 1) / scale;
+    const double d0 = (double)(HEAD - b0) * inv, d1 = (double)(HEAD - b1 - 1) * inv;
     const double slack = 4e-7 * (fabs(first) + fabs(d0) + fabs(d1));
     mid = (float)(first + 0.5 * (d0 + d1));
     half = b0 > b1 ? -1.0f : b1 == BINS - 1 ? INFINITY : (float)(0.5 * (d0 - d1) + slack);
@@ -655,15 +655,12 @@ __device__ __forceinline__ uint64_t block_before(uint64_t mine, unsigned long lo
   const uint64_t run = sum_lanes<64>(mine, threadIdx.x & 63);
   if ((threadIdx.x & 63) == 63) buf[threadIdx.x >> 6] = run;
   __syncthreads();
-  uint64_t sum = 0, before = 0;
-#pragma unroll
-  for (int w = 0; w < NT / 64; w++) {
-    if (w == (int)(threadIdx.x >> 6)) before = sum;
-    sum += buf[w];
-  }
-  all = sum;
+  constexpr int W = NT / 64;
+  const uint64_t waves = sum_lanes<W>((uint64_t)buf[threadIdx.x % W], threadIdx.x % W);
+  const int wave = uniform((int)threadIdx.x >> 6);
+  all = read_lane(waves, W - 1);
   __syncthreads();
-  return before + run - mine;
+  return (wave ? read_lane(waves, wave - 1) : 0) + run - mine;
 }
 
 // The first pass: counts and / or mantissas of every step.  Returns what only the row as a whole shows: its largest logit
@@ -742,7 +739,7 @@ template <typename T, bool MASKED, int NT>
 __device__ __noinline__ bool list_steps(int a0, int a1, int b0, int b1) {
   Long<NT>& g = shared<NT>();
   const Source<T, MASKED> src = shared_source<T, MASKED, NT>();
-  const Steps steps{uniform(g.steps.first), uniform(g.steps.scale), 0.0, uniform(g.steps.base)};
+  const Steps steps{uniform(g.steps.first), uniform(g.steps.scale), uniform(g.steps.inv), 0.0, uniform(g.steps.base)};
   a0 = uniform(a0), a1 = uniform(a1), b0 = uniform(b0), b1 = uniform(b1);
   if (threadIdx.x == 0) g.listed = 0;
   __syncthreads();
@@ -928,7 +925,9 @@ __device__ __forceinline__ uint64_t draw_by_steps(const Steps& steps, float top,
   int b0 = BINS, b1 = -1;
   if (o.top_p < 1) b0 = b1 = step_of(g, g.weight, border_of(o.top_p, sum));
   if (o.min_w > 0) {
-    const double lowest = (double)top + (o.min_p < 1 ? log(fmax(o.min_p, 1e-300)) / o.inv_t : 0.0);
+    double least = o.min_p;
+    asm volatile("" : "+v"(least));  // the logarithm stays here: every row would pay for it ahead of the passes
+    const double lowest = (double)top + (least < 1 ? log(fmax(least, 1e-300)) / o.inv_t : 0.0);
     const int m = Steps::of((steps.first - lowest) * steps.scale + HEAD);
     const int m0 = m > 1 ? m - 1 : 0, m1 = m + 1 < BINS ? m + 1 : BINS - 1;
     if (b1 < 0 || m1 < b0) {
@@ -1029,6 +1028,10 @@ __global__ __launch_bounds__(NT, 4) void sample_long(const T* logits, int64_t st
     if (threadIdx.x == 0) out[r] = wrong || !best ? -1 : column_of(best);
     return;
   }
+  for (int b = threadIdx.x; b < BINS; b += NT) {
+    g.count[b] = 0;
+    g.weight[b] = 0;
+  }
   // the first vectors: where the steps start and how narrow they can be
   const Source<T, MASKED> start{src.z, src.mask, cols < NT * (16 / (int)sizeof(T)) ? cols : NT * (16 / (int)sizeof(T))};
   float first = -INFINITY, least = INFINITY;
@@ -1044,10 +1047,6 @@ __global__ __launch_bounds__(NT, 4) void sample_long(const T* logits, int64_t st
         for (int i = 0; i < src.N; i++) look(c + i, v[i]);
       },
       look);
-  for (int b = threadIdx.x; b < BINS; b += NT) {
-    g.count[b] = 0;
-    g.weight[b] = 0;
-  }
   first = group_max<64>(first);
   least = -group_max<64>(-least);
   open = group_sum<64>(open);
@@ -1057,24 +1056,24 @@ __global__ __launch_bounds__(NT, 4) void sample_long(const T* logits, int64_t st
     g.wave[threadIdx.x >> 6] = open;
   }
   __syncthreads();
-  open = 0;
-  for (int w = 0; w < NT / 64; w++) {
-    first = fmaxf(first, g.fbuf[0][w]);
-    least = fminf(least, g.fbuf[1][w]);
-    open += (int)g.wave[w];
-  }
+  constexpr int W = NT / 64;
+  first = group_max<W>(g.fbuf[0][threadIdx.x % W]);
+  least = -group_max<W>(-g.fbuf[1][threadIdx.x % W]);
+  open = group_sum<W>((int)g.wave[threadIdx.x % W]);
   const bool counted = o.top_k > 0 && o.top_k < cols, weighed = !counted || o.top_k > Long<NT>::LISTED / 2;
   for (int turn = 0; turn < 2; turn++) {
     // a power of two of the weight in 32 steps; narrower where the first vectors (enough of them that are not barred) lie
     // within 1024 T counts as 2^-35 |first| at least: the next float32 below would still weigh e^-2048, and first * scale stays
     // below 2^41
-    const double most = 34359738368.0 / fabs((double)first), inv_t = fmin(o.inv_t, most);
-    const double close = open < 256 ? 0.0 : 1024.0 / ((double)first - (double)least);
+    // (to some 2^-20: they choose the scale, whose own bits are what counts)
+    const double most = 34359738368.0 * __builtin_amdgcn_rcp(fabs((double)first)), inv_t = fmin(o.inv_t, most);
+    const double close = open < 256 ? 0.0 : 1024.0 * __builtin_amdgcn_rcp((double)first - (double)least);
     const double wanted = fmin(fmin(fmax(fmax(32.0 * 1.4426950408889634 * inv_t, close), 1e-30), 64.0 * most), 1e300);
     Steps steps;
     steps.first = uniform(first);
     steps.scale = uniform(__longlong_as_double(__double_as_longlong(wanted) >> 37 << 37));
-    steps.width = uniform(inv_t / steps.scale);
+    steps.inv = uniform(1.0 / steps.scale);
+    steps.width = uniform(inv_t * steps.inv);
     steps.base = uniform(steps.first * steps.scale + HEAD);
     if (turn)
       for (int b = threadIdx.x; b < BINS; b += NT) {
