@@ -10,8 +10,8 @@
 // result depends on the order in which a launch happens to add, and a border that lies 2^-45 of the row's weight away is still
 // told apart (fp32 sums over 10^5 categories lose 2^-20 and would draw another category).
 //
-// Measured on an MI355X: 16384 x 2 fp32 3.4 us, 16384 x 1000 72, 1 x 32768 18, 37 x 50021 with a mask 30, 256 x 131072 bf16,
-// top_p 0.9, 61, of which reading it once would take 13.  Short rows are bound by their launch, rows of hundreds by the
+// Measured on an MI355X: 16384 x 2 fp32 3.4 us, 16384 x 1000 72, 1 x 32768 15, 37 x 50021 with a mask 25, 256 x 131072 bf16,
+// top_p 0.9, 56, of which reading it once would take 13.  Short rows are bound by their launch, rows of hundreds by the
 // instructions of sorting out one row each, long ones by float64 instructions (17 a logit) and a second read.
 #include <type_traits>
 
@@ -249,9 +249,9 @@ struct List {
 };
 
 // Sorts the first n places (the larger first) and sums their weights.  Up to 256, with as many threads as there are for
-// each, every place is compared with all (n^2 steps, but without a barrier between them: 200 places take 2 us, sorting them 9);
+// each, every place is compared with all (n^2 steps, but without a barrier between them: 200 places take 3 us, sorting them 9);
 // more are sorted by bitonic exchanges in LDS, where pairs that are at most 64 apart stay within the 128 places of one wave and
-// need no barrier.  A place of 0 is none.
+// need no barrier.  A place below 2^32 (above it is the logit, never 0) is none; up to n all places differ.
 template <int NT, int LN>
 __device__ __forceinline__ void sort_list(List<LN>& l, int n, float top, const Row& o) {
   constexpr int Q = NT > 256 ? NT / 256 : 1;  // threads for each place
@@ -259,21 +259,23 @@ __device__ __forceinline__ void sort_list(List<LN>& l, int n, float top, const R
     __syncthreads();
     if ((int)threadIdx.x < n) {
       const uint64_t p = l.place[threadIdx.x];
-      l.upto[threadIdx.x] = p ? weight_of(logit_of(p), top, o) : 0;
+      l.upto[threadIdx.x] = p >> 32 ? weight_of(logit_of(p), top, o) : 0;
     }
     __syncthreads();
     const int i = threadIdx.x / Q;
-    const uint64_t own = i < n ? l.place[i] : 0;
-    uint64_t sum = 0;
+    uint64_t own = 0, sum = 0;
     int before = 0;
-#pragma unroll 4
-    for (int k = threadIdx.x % Q; k < n; k += Q) {
-      const uint64_t p = l.place[k], w = l.upto[k];
-      sum += p >= own ? w : 0;
-      before += p > own || (p == own && k < i);  // (places of 0 are many)
+    if (i < n) {
+      own = l.place[i];
+#pragma unroll 8
+      for (int k = threadIdx.x % Q; k < n; k += Q) {
+        const uint64_t p = l.place[k], w = l.upto[k];
+        sum += p > own ? w : 0;
+        before += p > own;
+      }
+      sum = group_sum<Q>(sum) + l.upto[i];
+      before = group_sum<Q>(before);
     }
-    sum = group_sum<Q>(sum);
-    before = group_sum<Q>(before);
     __syncthreads();
     if (i < n && threadIdx.x % Q == 0) {
       l.place[before] = own;
@@ -308,7 +310,7 @@ __device__ __forceinline__ void sort_list(List<LN>& l, int n, float top, const R
   const int each = (m + NT - 1) / NT, first = threadIdx.x * each;
   uint64_t own = 0;
   for (int i = first; i < first + each && i < m; i++) {
-    own += l.place[i] ? weight_of(logit_of(l.place[i]), top, o) : 0;
+    own += l.place[i] >> 32 ? weight_of(logit_of(l.place[i]), top, o) : 0;
     l.upto[i] = own;
   }
   const uint64_t run = sum_lanes<64>(own, threadIdx.x & 63);
@@ -598,7 +600,8 @@ __global__ __launch_bounds__(256, R > 16 ? 2 : 4) void sample_wave(const T* logi
 // exp.  An equal logit weighs exactly as much: scale has 16 bits, which makes first * scale + HEAD, and with it t of the first
 // logit, exact.
 //
-// 256 rows of 131072 bf16, a CU each: first vectors 4 us, first pass 20, sums of steps 3, second pass and list 16, draw 4.
+// 256 rows of 131072 bf16, a CU each: first vectors 3 us, first pass 21, sums of steps 2, second pass 10 (7 TB/s over all CUs),
+// list 3, the rest 5.  What every thread does for the row as a whole is 16 waves' work: 100 operations take 0.7 us.
 constexpr int BINS = 2048, HEAD = 512, DIGIT = 11;
 
 struct Steps {
@@ -743,36 +746,40 @@ __device__ __noinline__ bool list_steps(int a0, int a1, int b0, int b1) {
   a0 = uniform(a0), a1 = uniform(a1), b0 = uniform(b0), b1 = uniform(b1);
   if (threadIdx.x == 0) g.listed = 0;
   __syncthreads();
-  // which step a logit lies in is computed only for those near the wanted ones
+  // those near the wanted steps are listed; the few that lie in a step beside them are then taken out, in parallel (looked at
+  // where they are found, each held up its wave: 37 x 50021 took 2.7 us longer)
   float am, ah, bm, bh;
   steps.around(a0, a1, am, ah);
   steps.around(b0, b1, bm, bh);
-  auto near = [&](float v) { return fabsf(v - am) <= ah || fabsf(v - bm) <= bh; };
   auto take = [&](int c, float v) {
-    const int b = steps(v);
-    if (v == -INFINITY || !((b >= a0 && b <= a1) || (b >= b0 && b <= b1))) return;
+    if (!(fabsf(v - am) <= ah || fabsf(v - bm) <= bh)) return;
     const int i = atomicAdd(&g.listed, 1);
     if (i < Long<NT>::LISTED) g.l.place[i] = place_of(v, c);
   };
   src.template vectors<NT, 4>(
       [&](int c, const float* v) {
-        bool any = false;
+        float a = fabsf(v[0] - am), b = fabsf(v[0] - bm);
 #pragma unroll
-        for (int i = 0; i < src.N; i++) any |= near(v[i]);
-        if (!any) return;
-        int hits = 0;
-#pragma unroll
-        for (int i = 0; i < src.N; i++) hits |= near(v[i]) ? 1 << i : 0;
-        for (; hits; hits &= hits - 1) {
-          const int i = c + __ffs(hits) - 1;
-          take(i, src(i));
+        for (int i = 1; i < src.N; i++) {
+          a = fminf(a, fabsf(v[i] - am));
+          b = fminf(b, fabsf(v[i] - bm));
         }
+        if (!(a <= ah || b <= bh)) return;
+#pragma unroll
+        for (int i = 0; i < src.N; i++) take(c + i, v[i]);
       },
       take);
   __syncthreads();
   const int n = uniform(g.listed);
   __syncthreads();  // all have read it: the next list begins by clearing it
   if (n > Long<NT>::LISTED) return false;
+  for (int i = threadIdx.x; i < n; i += NT) {
+    const float v = logit_of(g.l.place[i]);
+    const int b = steps(v);
+    if (v > -INFINITY && ((b >= a0 && b <= a1) || (b >= b0 && b <= b1))) continue;
+    g.l.place[i] = i;  // sorted behind the others
+    atomicSub(&g.listed, 1);
+  }
   sort_list<NT>(g.l, n, uniform(g.top), uniform(g.o));
   return true;
 }
