@@ -70,6 +70,32 @@ Tensor workspace(Args& a, int64_t bytes, const Tensor& like) {
   return t;
 }
 
+// A tensor that a node keeps.  What comes back may be another one (hooks on saved tensors pack and unpack as they like): its
+// values are taken in any layout, another shape, type or device is refused.
+struct Kept {
+  SavedVariable saved;
+  std::vector<int64_t> sizes;
+  at::ScalarType type;
+  at::Device device = at::kCPU;
+  bool defined = false;
+
+  void keep(const Tensor& t) {
+    saved = SavedVariable(t, false);
+    if (!(defined = t.defined())) return;
+    sizes = t.sizes().vec();
+    type = t.scalar_type();
+    device = t.device();
+  }
+  Tensor get() const {
+    const Tensor t = saved.unpack();
+    if (!defined) return t;
+    TORCH_CHECK(t.defined() && t.sizes() == at::IntArrayRef(sizes) && t.scalar_type() == type && t.device() == device,
+                "factorysim: a tensor kept for the backward pass was unpacked with another shape, type or device");
+    return t.dim() == 2 ? rows_of(t) : t.contiguous();
+  }
+  void drop() { saved.reset_data(); }
+};
+
 // a backward pass's results; differentiating them is refused, where a graph of them is being made
 variable_list once(variable_list out) {
   if (!at::GradMode::is_enabled()) return out;
@@ -86,14 +112,14 @@ void no_tangent(const Tensor& t) {
 
 // ------------------------------------------------------------------ layer norm
 struct LayerNormBackward : public torch::autograd::Node {
-  SavedVariable x, weight, stats;
+  Kept x, weight, stats;
   at::ScalarType param;
 
   variable_list apply(variable_list&& grads) override {
     std::lock_guard<std::mutex> lock(mutex_);
     variable_list out(3);
     if (!grads[0].defined()) return out;
-    const Tensor x_ = x.unpack(), w = weight.unpack(), s = stats.unpack(), dy = rows_of(grads[0]);
+    const Tensor x_ = x.get(), w = weight.get(), s = stats.get().contiguous(), dy = rows_of(grads[0]);
     const auto parameter = x_.options().dtype(param);
     if (task_should_compute_output(0)) out[0] = at::empty(x_.sizes(), x_.options());
     if (task_should_compute_output(1)) out[1] = at::empty({x_.size(1)}, parameter);
@@ -120,9 +146,9 @@ struct LayerNormBackward : public torch::autograd::Node {
   }
   void release_variables() override {
     std::lock_guard<std::mutex> lock(mutex_);
-    x.reset_data();
-    weight.reset_data();
-    stats.reset_data();
+    x.drop();
+    weight.drop();
+    stats.drop();
   }
   std::string name() const override { return "LayerNormBackward"; }
 };
@@ -155,9 +181,9 @@ Tensor layer_norm(const Tensor& x, const std::optional<Tensor>& weight, const st
   if (!graph) return y;
   auto node = std::shared_ptr<LayerNormBackward>(new LayerNormBackward(), torch::autograd::deleteNode);
   node->set_next_edges(torch::autograd::collect_next_edges(x, w, b));
-  node->x = SavedVariable(x, false);
-  node->weight = SavedVariable(w, false);
-  node->stats = SavedVariable(stats, false);
+  node->x.keep(x);
+  node->weight.keep(w);
+  node->stats.keep(stats);
   node->param = w.defined() ? w.scalar_type() : b.defined() ? b.scalar_type() : x.scalar_type();
   torch::autograd::set_history(y, node);
   return y;
@@ -184,14 +210,14 @@ fm_distill_args distill_args(const Tensor& z, const Tensor& index, const Tensor&
 }
 
 struct DistillBackward : public torch::autograd::Node {
-  SavedVariable z, index, teacher, stats;
+  Kept z, index, teacher, stats;
   double temperature;
 
   variable_list apply(variable_list&& grads) override {
     std::lock_guard<std::mutex> lock(mutex_);
     variable_list out(1);
     if (!grads[0].defined()) return out;
-    const Tensor z_ = z.unpack(), i = index.unpack(), t = teacher.unpack(), s = stats.unpack(), &g = grads[0];
+    const Tensor z_ = z.get(), i = index.get(), t = teacher.get(), s = stats.get().contiguous(), &g = grads[0];
     out[0] = at::empty(z_.sizes(), z_.options());
     fm_distill_args a = distill_args(z_, i, t, temperature);
     a.stats = (float*)data(s);
@@ -203,10 +229,10 @@ struct DistillBackward : public torch::autograd::Node {
   }
   void release_variables() override {
     std::lock_guard<std::mutex> lock(mutex_);
-    z.reset_data();
-    index.reset_data();
-    teacher.reset_data();
-    stats.reset_data();
+    z.drop();
+    index.drop();
+    teacher.drop();
+    stats.drop();
   }
   std::string name() const override { return "DistillBackward"; }
 };
@@ -226,10 +252,10 @@ Tensor distill_loss(const Tensor& z, const Tensor& index, const Tensor& teacher,
   if (!graph) return loss;
   auto node = std::shared_ptr<DistillBackward>(new DistillBackward(), torch::autograd::deleteNode);
   node->set_next_edges(torch::autograd::collect_next_edges(z));
-  node->z = SavedVariable(z, false);
-  node->index = SavedVariable(index, false);
-  node->teacher = SavedVariable(teacher, false);
-  node->stats = SavedVariable(stats, false);
+  node->z.keep(z);
+  node->index.keep(index);
+  node->teacher.keep(teacher);
+  node->stats.keep(stats);
   node->temperature = temperature;
   torch::autograd::set_history(loss, node);
   return loss;
