@@ -46,6 +46,13 @@ def _library():
     return _loaded
 
 
+@torch.compiler.assume_constant_result
+def _ready():
+    """the operators are registered: under torch.compile this runs while the call is traced"""
+    _library()
+    return True
+
+
 def _call(op, *args):
     try:
         return op(*args)
@@ -106,7 +113,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
         raise ValueError(f"eps is finite and not negative, got {eps}")
     w = weight if weight is None or weight.is_contiguous() else weight.contiguous()
     b = bias if bias is None or bias.is_contiguous() else bias.contiguous()
-    _library()
+    _ready()
     y = _call(torch.ops.factorysim.layer_norm, _rows(x), w, b, eps)
     return y if x.dim() == 2 else y.view(x.shape)
 
@@ -187,7 +194,7 @@ def sample_logits(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, mas
     if t != t or p != p or q != q:
         raise ValueError("temperature, top_p and min_p are numbers, not NaN")
     u = u.reshape(-1).contiguous() if u.dim() != 1 or not u.is_contiguous() else u
-    _library()
+    _ready()
     out = _call(torch.ops.factorysim.sample_logits, z, u, m, t, min(max(k, 0), 2**31 - 1), p, q, t_rows, k_rows, p_rows, q_rows)
     return out if logits.dim() == 2 else out.view(logits.shape[:-1])
 
@@ -218,6 +225,6 @@ def distill_loss(logits, teacher_index, teacher_logits, temperature=1.0):
     temperature = float(temperature)
     if not 1e-30 <= temperature <= 1e30:
         raise ValueError(f"temperature is positive and within 1e-30 .. 1e30, got {temperature}")
-    _library()
+    _ready()
     loss = _call(torch.ops.factorysim.distill_loss, _rows(logits), _rows(teacher_index), _rows(teacher_logits), temperature)
     return loss if logits.dim() == 2 else loss.view(logits.shape[:-1])

@@ -63,3 +63,105 @@ def test_other_tensors_unpacked_are_refused(change):
             with pytest.raises(RuntimeError, match="kept for the backward pass"):
                 y.backward(dy)
                 loss.backward(g)
+
+
+# ------------------------------------------------------------------ tracing
+def _bias_gradient(x, w, b, dy, z, at, t, g):
+    leaf = b.clone().requires_grad_()
+    return torch.autograd.grad(ops.layer_norm(x, None, leaf), leaf, dy)
+
+
+CALLS = {
+    "layer_norm": lambda x, w, b, dy, z, at, t, g: ops.layer_norm(x, w, b),
+    "layer_norm without parameters": lambda x, w, b, dy, z, at, t, g: ops.layer_norm(x[:, None, 1:]),
+    "sample_logits": lambda x, w, b, dy, z, at, t, g: ops.sample_logits(z, g.abs() % 1, top_p=0.9, top_k=g.long().abs() + 1),
+    "sample_logits, mask": lambda x, w, b, dy, z, at, t, g: ops.sample_logits(z, g.abs() % 1, mask=b > 0),
+    "distill_loss": lambda x, w, b, dy, z, at, t, g: ops.distill_loss(z, at, t, temperature=2.0),
+    "gradients": gradients,
+    "bias only": _bias_gradient,
+}
+
+
+def same(a, b):
+    a, b = ([v] if torch.is_tensor(v) else list(v) for v in (a, b))
+    return len(a) == len(b) and all(p.dtype == q.dtype and torch.equal(p, q) for p, q in zip(a, b))
+
+
+def other_inputs(device=CPU):
+    x, w, b, dy, z, at, t, g = inputs(device)
+    return x.flip(0) + 1, w.flip(0), b.flip(0) - 0.1, dy.flip(1), z.flip(1) * 2, at.flip(0), t.flip(1), g.flip(0)
+
+
+@pytest.mark.parametrize("mode", ["real", "fake", "symbolic"])
+@pytest.mark.parametrize("call", list(CALLS))
+def test_traced_calls_compute_what_they_recorded(call, mode):
+    """a recorded graph holds the operators: on new inputs it gives what a call gives"""
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    graph = make_fx(CALLS[call], tracing_mode=mode)(*inputs())
+    assert any("factorysim" in str(n.target) for n in graph.graph.nodes)
+    for args in (inputs(), other_inputs()):
+        assert same(graph(*args), CALLS[call](*args))
+
+
+@pytest.mark.parametrize("call", ["layer_norm", "layer_norm without parameters", "distill_loss"])
+def test_traced_graphs_are_differentiable_again(call):
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    graph = make_fx(CALLS[call])(*inputs())
+    args, again = list(inputs()), list(inputs())
+    for a in (args, again):
+        for i in (0, 1, 2, 4):
+            a[i].requires_grad_()
+    out, want = graph(*args), CALLS[call](*again)
+    out.sum().backward(), want.sum().backward()
+    for a, b in zip(args, again):
+        assert (a.grad is None) == (b.grad is None) and (a.grad is None or torch.equal(a.grad, b.grad))
+
+
+@pytest.mark.parametrize("dynamic", [False, True])
+def test_compiled_calls(dynamic):
+    torch._dynamo.reset()
+
+    def step(x, w, b, z, at, t, u):
+        y = ops.layer_norm(x, w, b)
+        return y.tanh(), ops.distill_loss(z + y, at, t, temperature=2.0), ops.sample_logits(z, u, top_p=0.9)
+
+    compiled = torch.compile(step, backend="aot_eager", fullgraph=True, dynamic=dynamic)
+    for rows in (4, 3):
+        results = []
+        for f in (step, compiled):
+            x, w, b, _, z, at, t, g = inputs()
+            leaves = [v[:rows].clone().requires_grad_() for v in (x, z)] + [v.clone().requires_grad_() for v in (w, b)]
+            y, loss, token = f(leaves[0], leaves[2], leaves[3], leaves[1], at[:rows], t[:rows], g[:rows].abs() % 1)
+            results.append([y.detach(), loss.detach(), token, *torch.autograd.grad((y.sum(1) * loss).sum(), leaves)])
+        assert same(*results)
+
+
+def test_a_compiled_call_may_be_the_first_one(monkeypatch):
+    torch._dynamo.reset()
+    monkeypatch.setattr(ops, "_loaded", None)  # as before anything was called
+    x = inputs()[0]
+    assert torch.equal(torch.compile(lambda v: ops.layer_norm(v), backend="eager", fullgraph=True)(x), ops.layer_norm(x))
+
+
+def test_registrations():
+    """torch's own check of an operator: schema, gradients, shapes without data, tracing"""
+    x, w, b, dy, z, at, t, g = inputs()
+    f = torch.ops.factorysim
+    for grad in (False, True):
+        xs, ws, bs, zs = (v.clone().requires_grad_(grad) for v in (x, w, b, z))
+        torch.library.opcheck(f.layer_norm.default, (xs, ws, bs, 1e-5))
+        torch.library.opcheck(f.layer_norm.default, (xs, None, None, 1e-5))
+        torch.library.opcheck(f.distill_loss.default, (zs, at, t, 1.5))
+        torch.library.opcheck(f.sample_logits.default, (zs, g.abs() % 1, None, 1.0, 0, 0.9, 0.0, None, None, None, None))
+
+
+def test_function_transforms():
+    x, w, b, dy, z, at, t, g = inputs()
+    a = x.clone().requires_grad_()
+    want, = torch.autograd.grad((ops.layer_norm(a, w, b) * dy).sum(), a)
+    assert torch.equal(torch.func.grad(lambda v: (ops.layer_norm(v, w, b) * dy).sum())(x), want)
+    stack = torch.stack([x, x + 1, 2 * x])
+    assert torch.equal(torch.func.vmap(lambda v: ops.layer_norm(v, w, b))(stack), ops.layer_norm(stack, w, b))
+    assert torch.equal(torch.func.vmap(lambda v: ops.distill_loss(v, at, t))(stack), torch.stack([ops.distill_loss(v, at, t) for v in stack]))
