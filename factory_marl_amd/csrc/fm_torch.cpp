@@ -1,7 +1,7 @@
 // fm_torch.cpp -- the operators' calls from tensors: factory_marl_amd/ops.py checks and shapes the arguments and calls
 // torch.ops.factorysim.*, whose backward passes run here without the interpreter (a Python node waits for it on the
 // engine's thread: a layer norm of 64 x 128, forward and backward, took 105 us of host time with one and takes 60 like this).
-// All computing is the library's; its entry points are handed over once, by `bind`.
+// All computing is the library's; its entry points are handed over once, by fm_torch_bind.
 //
 // Each operator is registered for the dispatch keys that it has a form of its own for: CPU and CUDA compute, Meta gives the
 // results' shapes, Autograd makes the graph and calls what is below it through the dispatcher again.  So whatever stands
@@ -16,8 +16,10 @@
 #include <torch/csrc/autograd/saved_variable.h>
 #include <torch/library.h>
 
+#include <algorithm>
 #include <array>
 #include <cstring>
+#include <initializer_list>
 #include <optional>
 #include <tuple>
 #include <vector>
@@ -40,11 +42,6 @@ struct Entries {
   decltype(&fm_sample_workspace) sample_workspace;
   decltype(&fm_last_error) last_error;
 } fm;
-
-void bind(at::IntArrayRef addresses) {
-  TORCH_CHECK(addresses.size() * sizeof(void*) == sizeof(fm), "factorysim: entry points");
-  std::memcpy(&fm, addresses.data(), sizeof(fm));
-}
 
 void check(int rc) { TORCH_CHECK(rc == 0, "factorysim error ", rc, ": ", fm.last_error()); }
 
@@ -72,6 +69,21 @@ void* data(const Tensor& t) { return t.defined() && t.numel() ? t.data_ptr() : n
 
 // [rows, cols] with adjacent columns
 Tensor rows_of(const Tensor& t) { return t.size(1) <= 1 || t.stride(1) == 1 ? t : t.contiguous(); }
+
+// A call's arguments are checked here too, since the operators can be called directly: kernels read and write what these say.
+// t: on x's device, of these sizes, of one of the types
+void need(const char* name, const Tensor& t, const Tensor& x, at::IntArrayRef sizes, std::initializer_list<at::ScalarType> types) {
+  TORCH_CHECK(t.device() == x.device(), "factorysim: ", name, " is on ", t.device(), ", the first input on ", x.device());
+  TORCH_CHECK(t.sizes() == sizes, "factorysim: ", name, " has shape ", t.sizes(), ", not ", sizes);
+  TORCH_CHECK_TYPE(std::find(types.begin(), types.end(), t.scalar_type()) != types.end(), "factorysim: ", name, " is ",
+                   t.scalar_type());
+}
+void need_rows(const char* name, const Tensor& x) {
+  TORCH_CHECK(x.dim() == 2 && x.size(1) > 0, "factorysim: ", name, " is [rows, columns], not ", x.sizes());
+}
+void need_parameter(const char* name, const std::optional<Tensor>& p, const Tensor& x) {
+  if (p) need(name, *p, x, {x.size(1)}, {x.scalar_type(), at::kFloat});
+}
 
 template <typename Args>
 Tensor workspace(Args& a, int64_t bytes, const Tensor& like) {
@@ -146,6 +158,10 @@ Tensor or_none(const Maybe& t) { return t.value_or(Tensor()); }
 // ------------------------------------------------------------------ computing (CPU, CUDA)
 // Rows are [rows, cols], as tensors of any layout.
 Tensor norm_run(const Tensor& x_, const Maybe& weight, const Maybe& bias, double eps, Tensor* stats) {
+  need_rows("x", x_);
+  need_parameter("weight", weight, x_);
+  need_parameter("bias", bias, x_);
+  TORCH_CHECK_TYPE(!weight || !bias || weight->scalar_type() == bias->scalar_type(), "factorysim: weight and bias differ in type");
   const Tensor x = rows_of(x_), w = weight ? weight->contiguous() : Tensor(), b = bias ? bias->contiguous() : Tensor();
   const int64_t n = x.size(0);
   Tensor y = at::empty({n, x.size(1)}, x.options());
@@ -184,6 +200,11 @@ Two layer_norm_stats(const Tensor& x, const Maybe& weight, const Maybe& bias, do
 // of dx, dweight, dbias (of type param) those that are wanted
 std::vector<Tensor> layer_norm_backward(const Tensor& dy_, const Tensor& x_, const Maybe& weight, const Tensor& stats,
                                         at::ScalarType param, Three wanted) {
+  need_rows("x", x_);
+  need("dy", dy_, x_, x_.sizes(), {x_.scalar_type()});
+  need("stats", stats, x_, {2, x_.size(0)}, {at::kFloat});
+  TORCH_CHECK_TYPE(param == x_.scalar_type() || param == at::kFloat, "factorysim: param is float32 or x's type");
+  if (weight) need("weight", *weight, x_, {x_.size(1)}, {param});
   const Tensor x = rows_of(x_), dy = rows_of(dy_), s = stats.contiguous(), w = weight ? weight->contiguous() : Tensor();
   const auto parameter = x.options().dtype(param);
   Tensor dx, dw, db;
@@ -214,6 +235,13 @@ std::vector<Tensor> layer_norm_backward(const Tensor& dy_, const Tensor& x_, con
   return out;
 }
 
+void check_distill(const Tensor& z, const Tensor& index, const Tensor& teacher) {
+  need_rows("logits", z);
+  need_rows("teacher_index", index);
+  need("teacher_index", index, z, {z.size(0), index.size(1)}, {at::kInt, at::kLong});
+  need("teacher_logits", teacher, z, index.sizes(), {at::kFloat, at::kHalf, at::kBFloat16});
+}
+
 fm_distill_args distill_args(const Tensor& z, const Tensor& index, const Tensor& teacher, double temperature) {
   fm_distill_args a = {};
   place(a, z);
@@ -234,6 +262,7 @@ fm_distill_args distill_args(const Tensor& z, const Tensor& index, const Tensor&
 }
 
 Tensor distill_run(const Tensor& z_, const Tensor& index_, const Tensor& teacher_, double temperature, Tensor* stats) {
+  check_distill(z_, index_, teacher_);
   const Tensor z = rows_of(z_), index = rows_of(index_), teacher = rows_of(teacher_);
   fm_distill_args a = distill_args(z, index, teacher, temperature);
   const auto floats = z.options().dtype(at::kFloat);
@@ -261,6 +290,9 @@ Two distill_loss_stats(const Tensor& z, const Tensor& index, const Tensor& teach
 
 Tensor distill_backward(const Tensor& grad, const Tensor& z_, const Tensor& index_, const Tensor& teacher_, const Tensor& stats,
                         double temperature) {
+  check_distill(z_, index_, teacher_);
+  need("grad", grad, z_, {z_.size(0)}, {at::kFloat});
+  need("stats", stats, z_, {z_.size(0), 2}, {at::kFloat});
   const Tensor z = rows_of(z_), index = rows_of(index_), teacher = rows_of(teacher_), s = stats.contiguous();
   Tensor dz = at::empty(z.sizes(), z.options());
   fm_distill_args a = distill_args(z, index, teacher, temperature);
@@ -276,6 +308,14 @@ Tensor distill_backward(const Tensor& grad, const Tensor& z_, const Tensor& inde
 Tensor sample_logits(const Tensor& z_, const Tensor& u_, const Maybe& mask_, double temperature, int64_t top_k, double top_p,
                      double min_p, const Maybe& temperature_rows, const Maybe& top_k_rows, const Maybe& top_p_rows,
                      const Maybe& min_p_rows) {
+  need_rows("logits", z_);
+  const int64_t n = z_.size(0);
+  need("u", u_, z_, {n}, {at::kFloat, at::kDouble});
+  if (mask_) need("mask", *mask_, z_, {mask_->dim() && mask_->size(0) == 1 ? 1 : n, z_.size(1)}, {at::kBool});
+  if (temperature_rows) need("temperature", *temperature_rows, z_, {n}, {at::kFloat});
+  if (top_k_rows) need("top_k", *top_k_rows, z_, {n}, {at::kInt});
+  if (top_p_rows) need("top_p", *top_p_rows, z_, {n}, {at::kFloat});
+  if (min_p_rows) need("min_p", *min_p_rows, z_, {n}, {at::kFloat});
   const Tensor z = rows_of(z_), u = u_.contiguous(), mask = mask_ ? rows_of(*mask_) : Tensor();
   auto flat = [](const Maybe& t) { return t ? t->contiguous() : Tensor(); };
   const Tensor t_rows = flat(temperature_rows), k_rows = flat(top_k_rows), p_rows = flat(top_p_rows), m_rows = flat(min_p_rows);
@@ -283,7 +323,7 @@ Tensor sample_logits(const Tensor& z_, const Tensor& u_, const Maybe& mask_, dou
   place(a, z);
   a.dtype = code(z);
   a.u_dtype = u.scalar_type() == at::kDouble ? FM_DTYPE_F64 : FM_DTYPE_F32;
-  a.rows = z.size(0);
+  a.rows = n;
   a.cols = z.size(1);
   a.logits = data(z);
   a.stride = row_stride(z);
@@ -468,8 +508,14 @@ Tensor distill_backward(const Tensor& grad, const Tensor& z, const Tensor& index
 }  // namespace graph
 }  // namespace
 
+// the library's entry points, in the order of Entries; false: not as many
+extern "C" bool fm_torch_bind(void* const* addresses, int64_t count) {
+  if (count * sizeof(void*) != sizeof(fm)) return false;
+  std::memcpy(&fm, addresses, sizeof(fm));
+  return true;
+}
+
 TORCH_LIBRARY(factorysim, m) {
-  m.def("bind(int[] addresses) -> ()", &bind);
   m.def("layer_norm(Tensor x, Tensor? weight, Tensor? bias, float eps) -> Tensor");
   m.def("layer_norm_stats(Tensor x, Tensor? weight, Tensor? bias, float eps) -> (Tensor, Tensor)");
   m.def("layer_norm_backward(Tensor dy, Tensor x, Tensor? weight, Tensor stats, ScalarType param, bool[3] wanted) -> Tensor[]");

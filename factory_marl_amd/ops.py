@@ -41,7 +41,11 @@ def _library():
         torch.ops.load_library(_NODES)
         names = ("fm_layer_norm_forward", "fm_layer_norm_backward", "fm_layer_norm_workspace", "fm_distill_forward",
                  "fm_distill_backward", "fm_distill_workspace", "fm_sample_logits", "fm_sample_workspace", "fm_last_error")
-        torch.ops.factorysim.bind([C.cast(getattr(L, n), C.c_void_p).value for n in names])
+        addresses = (C.c_void_p * len(names))(*(C.cast(getattr(L, n), C.c_void_p).value for n in names))
+        bind = C.CDLL(_NODES).fm_torch_bind
+        bind.argtypes, bind.restype = [C.POINTER(C.c_void_p), C.c_int64], C.c_bool
+        if not bind(addresses, len(names)):
+            raise _lib.FactorySimError(f"{_NODES} is of another version than {_lib.LIB_PATH}: rebuild both")
         _loaded = L
     return _loaded
 

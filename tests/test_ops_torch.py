@@ -148,6 +148,7 @@ def test_a_compiled_call_may_be_the_first_one(monkeypatch):
 def test_registrations():
     """torch's own check of an operator: schema, gradients, shapes without data, tracing"""
     x, w, b, dy, z, at, t, g = inputs()
+    ops._library()
     f = torch.ops.factorysim
     for grad in (False, True):
         xs, ws, bs, zs = (v.clone().requires_grad_(grad) for v in (x, w, b, z))
@@ -165,3 +166,45 @@ def test_function_transforms():
     stack = torch.stack([x, x + 1, 2 * x])
     assert torch.equal(torch.func.vmap(lambda v: ops.layer_norm(v, w, b))(stack), ops.layer_norm(stack, w, b))
     assert torch.equal(torch.func.vmap(lambda v: ops.distill_loss(v, at, t))(stack), torch.stack([ops.distill_loss(v, at, t) for v in stack]))
+
+
+# ------------------------------------------------------------------ the registered operators, called directly
+def test_direct_calls_are_checked():
+    """whatever would be read or written past its end, or on another device, is refused"""
+    x, w, b, dy, z, at, t, g = inputs()
+    ops._library()
+    f = torch.ops.factorysim
+    u, stats, dstats = g.abs() % 1, torch.rand(2, 4), torch.rand(4, 2)
+    calls = [
+        (f.layer_norm, [x, w, b, 1e-5]), (f.layer_norm_stats, [x, w, b, 1e-5]),
+        (f.layer_norm_backward, [dy, x, w, stats, torch.float32, [True] * 3]),
+        (f.distill_loss, [z, at, t, 1.0]), (f.distill_loss_stats, [z, at, t, 1.0]), (f.distill_backward, [g, z, at, t, dstats, 1.0]),
+        (f.sample_logits, [z, u, z > 0, 1.0, 0, 1.0, 0.0, u, at[:, 0].int(), u, u]),
+    ]
+    for op, args in calls:
+        op(*args)
+        for i, a in enumerate(args):
+            if not torch.is_tensor(a):
+                continue
+            for bad in (a[:-1], a[..., :-1], a[None], a.reshape(-1), a.to(torch.float64 if a.dtype != torch.float64 else torch.float32),
+                        a.to(torch.complex64), a.new_empty(0)):
+                if bad.shape == a.shape and (bad.dtype == a.dtype or op is f.sample_logits and i == 1):
+                    continue
+                if op in (f.layer_norm, f.layer_norm_stats) and a is x and bad.shape == (3, 6) or \
+                        op in (f.distill_loss, f.distill_loss_stats, f.distill_backward) and a is z and bad.shape == (4, 5):
+                    continue  # fewer rows or columns: this argument alone says how many
+                with pytest.raises((RuntimeError, TypeError)):
+                    op(*args[:i], bad, *args[i + 1:])
+    for args in ([x.half(), w, b.half(), 1e-5], [x.half(), w.bfloat16(), None, 1e-5], [x[:, :0], None, None, 1e-5]):
+        with pytest.raises((RuntimeError, TypeError)):
+            f.layer_norm(*args)
+    with pytest.raises(RuntimeError):
+        f.layer_norm_backward(dy, x, w, stats, torch.float16, [True] * 3)
+    broad = f.sample_logits(z, u, (z > 0)[:1], 1.0, 0, 1.0, 0.0, None, None, None, None)  # one row of a mask for all
+    assert torch.equal(broad, ops.sample_logits(z, u, mask=(z > 0)[0]))
+
+
+def test_the_entry_points_are_no_operator():
+    ops._library()
+    with pytest.raises(AttributeError):
+        torch.ops.factorysim.bind
