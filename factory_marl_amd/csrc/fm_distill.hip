@@ -428,9 +428,6 @@ bool with_group(int64_t cols, int64_t k, F&& f) {
   return true;
 }
 
-// n blocks as a grid that holds any number of them
-dim3 grid_of(int64_t n) { return dim3((unsigned)(n < (1 << 20) ? n : 1 << 20), (unsigned)((n + (1 << 20) - 1) >> 20)); }
-
 template <typename T>
 void forward(const fm_distill_args& a) {
   hipStream_t st = (hipStream_t)a.stream;

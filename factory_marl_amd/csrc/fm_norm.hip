@@ -397,8 +397,10 @@ __global__ __launch_bounds__(ST) void norm_dparam_sum(const float* part, int par
   constexpr int LANES = ST * C / 64;
   __shared__ float buf[LANES][65];
   // over dweight's and dbias's columns in turn
-  const int all = 2 * cols, c = threadIdx.x % (64 / C) * C, lane = threadIdx.x / (64 / C);
-  const int o = blockIdx.x * 64 + c, at = o < all - C ? o : all - C;
+  const int all = 2 * cols, from = (int)(blockIdx.x + gridDim.x * blockIdx.y) * 64;
+  if (from >= all) return;
+  const int c = threadIdx.x % (64 / C) * C, lane = threadIdx.x / (64 / C);
+  const int o = from + c, at = o < all - C ? o : all - C;
   float s[C] = {};
 #pragma unroll 8
   for (int p = lane; p < parts; p += LANES) {
@@ -416,7 +418,7 @@ __global__ __launch_bounds__(ST) void norm_dparam_sum(const float* part, int par
 #pragma unroll
   for (int i = k; i < LANES; i += 16) a += buf[i][d];
   a = group_sum<16>(a);
-  const int od = blockIdx.x * 64 + d / C * C;  // as at, of column d
+  const int od = from + d / C * C;  // as at, of column d
   const int to = (od < all - C ? od : all - C) + d % C;
   if (k == 0) {
     if (to < cols && dweight) dweight[to] = from_f32<P>(a);
@@ -506,7 +508,7 @@ void backward(const fm_layer_norm_args& a) {
   }
   if (!sums) return;
   if (cols > 1)
-    norm_dparam_sum<P, 4><<<(2 * cols + 63) / 64, ST, 0,
+    norm_dparam_sum<P, 4><<<grid_of((2 * (int64_t)cols + 63) / 64), ST, 0,
         st>>>((const float*)a.workspace, parts, (P*)a.dweight, (P*)a.dbias, cols);
   else
     norm_dparam_sum<P, 1><<<1, ST, 0, st>>>((const float*)a.workspace, parts, (P*)a.dweight, (P*)a.dbias, cols);

@@ -125,6 +125,11 @@ __device__ __forceinline__ float block_max(float v, float* buf) {
   return group_max<NT / 64>(buf[threadIdx.x % (NT / 64)]);
 }
 
+// n blocks as a grid that holds any number of them: a grid's line is limited to 2^32 threads
+inline dim3 grid_of(int64_t n) {
+  return dim3((unsigned)(n < (1 << 20) ? n : 1 << 20), (unsigned)((n + (1 << 20) - 1) >> 20));
+}
+
 // Makes `device` current for one call's launches and restores the caller's; status() reports what the launches did.
 struct OnDevice {
   int before = -1;
