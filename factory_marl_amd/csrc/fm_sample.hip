@@ -597,8 +597,7 @@ __global__ __launch_bounds__(256, R > 16 ? 2 : 4) void sample_wave(const T* logi
 // - v) scale + HEAD, step b = floor(t) and r = t - b, a category weighs exp(-r width) times what the top of its step does,
 // width = 1 / (scale T) <= 0.022 (32 steps to a power of two; more where the first vectors are closer together).  A polynomial
 // of degree 4 in r gives that to 5e-13 (four operations, 15 with the step's), and only the steps' sums are scaled by a proper
-// exp.  An equal logit weighs exactly as much: scale has 16 bits, which makes first * scale + HEAD, and with it t of the first
-// logit, exact.
+// exp.  Equal logits weigh the same, but not quite what a list's weigh: draw_by_steps takes care where that could show.
 //
 // 256 rows of 131072 bf16, a CU each: first vectors 3 us, first pass 21, sums of steps 2, second pass 10 (7 TB/s over all CUs),
 // list 3, the rest 5.  What every thread does for the row as a whole is 16 waves' work: 100 operations take 0.7 us.
@@ -919,7 +918,8 @@ __device__ __forceinline__ uint64_t draw_by_steps(const Steps& steps, float top,
     return draw_from<NT>(g.l, g.listed, o);
   }
   const int b = cut ? step_of(g, g.count, (uint64_t)o.top_k - 1) : BINS - 1;
-  if (cut && !(b == BINS - 1 && steps.past())) {
+  const bool shorter = cut && !(b == BINS - 1 && steps.past());
+  if (shorter) {
     if (!list_steps<T, MASKED, NT>(b, b, 0, -1)) return 0;
     const int i = (int)(o.top_k - 1 - g.count[b]);
     if (!g.listed) return 0;
@@ -969,6 +969,11 @@ __device__ __forceinline__ uint64_t draw_by_steps(const Steps& steps, float top,
         split = g.step;
         __syncthreads();
       }
+      // Where the list holds all that weighs, the row's sum is the list's, in which equal logits weigh exactly as much.  The
+      // steps' sums are off by up to 5e-13 of themselves: a share of 256 equal logits' weight could end one of them later.
+      if (together && !shorter && g.weight[joined ? (t0 < b0 ? t0 : b0) : t0] == 0 &&
+          g.weight[(border ? b1 : t1) + 1] == all && (!border || joined || g.weight[t1 + 1] == g.weight[b0]) && g.listed)
+        sum = g.l.upto[g.listed - 1];
       const uint64_t off = split ? g.l.upto[split - 1] : 0;  // of the list's sum, what belongs to the draw's steps
       if (border) {
         int end = g.listed;  // what is kept of the list

@@ -28,3 +28,38 @@ def test_parameter_gradients_of_the_widest_rows(cols):
         h = (x[0, at].double() - mean) * torch.rsqrt(var + 1e-5)
         want, slack = dy[0, at].double() * h, dy[0, at].double().abs() * lost * (size + h.abs())
         assert ((dw[at].double() - want).abs() <= slack + 2.0**-11 * (want.abs() + slack) + 2.0**-25).all()
+
+
+@pytest.mark.parametrize("kind,cols", [("f32", 4100), ("f32", 8192), ("f32", 16383), ("f16", 8200), ("bf16", 16384)])
+def test_norm_blocks_of_512_and_1024_threads_go_on_to_later_rows(kind, cols):
+    """a row a block of one CU: with 300 rows some blocks take two, one with and one without a row to follow"""
+    t = cases.DTYPES[kind]
+    cases.check_norm(*cases.norm_inputs(300, cols, t, t, DEV))
+
+
+def test_norm_wide_rows_beyond_the_sums_of_one_stretch():
+    """more than 16 rows a stretch of the parameters' sums, and more rows than one a block"""
+    cases.check_norm(*cases.norm_inputs(600, 16400, torch.bfloat16, torch.float32, DEV))
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,cols", [(200, 1500), (200, 2100), (200, 9001), (1100, 5003), (100, 70001)])
+def test_draws_exactly_on_the_borders_of_equal_logits(rows, cols, kind):
+    """256 equal logits, whatever they are, and nothing else that weighs: u = k / 256 draws the k-th of them, and of the half
+    that top_p = 0.5 keeps u = k / 128 (the first up to which MORE than u of the weight lies); top_p = n / 256 keeps n"""
+    g = torch.Generator().manual_seed(cols)
+    for rest in (-float("inf"), -1e4):
+        at = torch.stack([torch.randperm(cols, generator=g)[:256] for _ in range(rows)]).sort(1).values
+        value = torch.cat([1e-3 * torch.randn(rows // 2, generator=g), 10 * torch.randn(rows - rows // 2, generator=g)])
+        z = torch.full((rows, cols), rest).scatter_(1, at, value[:, None].expand(rows, 256)).to(DEV, cases.DTYPES[kind])
+        k = torch.randint(0, 128, (rows,), generator=g)
+        want = at.gather(1, k[:, None])[:, 0]
+        for settings, parts in ((dict(), 256), (dict(top_p=0.5), 128), (dict(min_p=1.0), 256), (dict(top_k=128), 128), (dict(temperature=0.3), 256)):
+            got = ops.sample_logits(z, (k / parts).to(DEV), **settings)
+            assert torch.equal(got.cpu(), want), (rest, settings, int((got.cpu() != want).sum()))
+        for p in (0.25, 0.5, 0.75):  # the last one kept
+            got = ops.sample_logits(z, torch.full((rows,), 1 - 2.0**-24, device=DEV), top_p=p).cpu()
+            assert torch.equal(got, at[:, int(256 * p) - 1]), (rest, p, int((got != at[:, int(256 * p) - 1]).sum()))
+        mask = torch.zeros(rows, cols, dtype=torch.bool).scatter_(1, at, True)
+        got = ops.sample_logits(value[:, None].expand(rows, cols).contiguous().to(DEV, cases.DTYPES[kind]), (k / 256).to(DEV), mask=mask.to(DEV))
+        assert torch.equal(got.cpu(), want)
