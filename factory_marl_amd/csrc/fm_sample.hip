@@ -750,24 +750,37 @@ __device__ __noinline__ bool list_steps(int a0, int a1, int b0, int b1) {
   float am, ah, bm, bh;
   steps.around(a0, a1, am, ah);
   steps.around(b0, b1, bm, bh);
+  const bool below = (a1 == BINS - 1 && a0 > 0 && a0 <= a1) || (b1 == BINS - 1 && b0 > 0 && b0 <= b1);
   auto take = [&](int c, float v) {
     if (!(fabsf(v - am) <= ah || fabsf(v - bm) <= bh)) return;
     const int i = atomicAdd(&g.listed, 1);
     if (i < Long<NT>::LISTED) g.l.place[i] = place_of(v, c);
   };
-  src.template vectors<NT, 4>(
-      [&](int c, const float* v) {
-        float a = fabsf(v[0] - am), b = fabsf(v[0] - bm);
+  if (below) {
+    // the last step, which has no lower end to be near to, but not all: each category's step (rare: it can still weigh only
+    // where the first vectors are much closer together than the rest)
+    src.template each<NT>([&](int c, float v) {
+      const int b = steps(v);
+      if (v > -INFINITY && ((b >= a0 && b <= a1) || (b >= b0 && b <= b1))) {
+        const int i = atomicAdd(&g.listed, 1);
+        if (i < Long<NT>::LISTED) g.l.place[i] = place_of(v, c);
+      }
+    });
+  } else {
+    src.template vectors<NT, 4>(
+        [&](int c, const float* v) {
+          float a = fabsf(v[0] - am), b = fabsf(v[0] - bm);
 #pragma unroll
-        for (int i = 1; i < src.N; i++) {
-          a = fminf(a, fabsf(v[i] - am));
-          b = fminf(b, fabsf(v[i] - bm));
-        }
-        if (!(a <= ah || b <= bh)) return;
+          for (int i = 1; i < src.N; i++) {
+            a = fminf(a, fabsf(v[i] - am));
+            b = fminf(b, fabsf(v[i] - bm));
+          }
+          if (!(a <= ah || b <= bh)) return;
 #pragma unroll
-        for (int i = 0; i < src.N; i++) take(c + i, v[i]);
-      },
-      take);
+          for (int i = 0; i < src.N; i++) take(c + i, v[i]);
+        },
+        take);
+  }
   __syncthreads();
   const int n = uniform(g.listed);
   __syncthreads();  // all have read it: the next list begins by clearing it
@@ -937,7 +950,9 @@ __device__ __forceinline__ uint64_t draw_by_steps(const Steps& steps, float top,
     const double lowest = (double)top + (least < 1 ? log(fmax(least, 1e-300)) / o.inv_t : 0.0);
     const int m = Steps::of((steps.first - lowest) * steps.scale + HEAD);
     const int m0 = m > 1 ? m - 1 : 0, m1 = m + 1 < BINS ? m + 1 : BINS - 1;
-    if (b1 < 0 || m1 < b0) {
+    if (g.weight[m0] >= sum) {
+      // all that is kept weighs more than that: no border (its list would often be the last step's, all that lies below)
+    } else if (b1 < 0 || m1 < b0) {
       b0 = m0;
       b1 = m1;
     } else if (m0 <= b1) {
@@ -971,8 +986,9 @@ __device__ __forceinline__ uint64_t draw_by_steps(const Steps& steps, float top,
       }
       // Where the list holds all that weighs, the row's sum is the list's, in which equal logits weigh exactly as much.  The
       // steps' sums are off by up to 5e-13 of themselves: a share of 256 equal logits' weight could end one of them later.
-      if (together && !shorter && g.weight[joined ? (t0 < b0 ? t0 : b0) : t0] == 0 &&
-          g.weight[(border ? b1 : t1) + 1] == all && (!border || joined || g.weight[t1 + 1] == g.weight[b0]) && g.listed)
+      if (together && g.weight[joined ? (t0 < b0 ? t0 : b0) : t0] == 0 && !shorter &&
+          g.weight[(border ? b1 : t1) + 1] == g.weight[BINS] && (!border || joined || g.weight[t1 + 1] == g.weight[b0]) &&
+          g.listed)
         sum = g.l.upto[g.listed - 1];
       const uint64_t off = split ? g.l.upto[split - 1] : 0;  // of the list's sum, what belongs to the draw's steps
       if (border) {

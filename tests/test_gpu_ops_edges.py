@@ -63,3 +63,46 @@ def test_draws_exactly_on_the_borders_of_equal_logits(rows, cols, kind):
         mask = torch.zeros(rows, cols, dtype=torch.bool).scatter_(1, at, True)
         got = ops.sample_logits(value[:, None].expand(rows, cols).contiguous().to(DEV, cases.DTYPES[kind]), (k / 256).to(DEV), mask=mask.to(DEV))
         assert torch.equal(got.cpu(), want)
+
+
+def milliseconds(call):
+    """the shortest of several runs of 5"""
+    call()
+    times = []
+    for _ in range(8):
+        a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        a.record()
+        for _ in range(5):
+            call()
+        b.record()
+        torch.cuda.synchronize(DEV)
+        times.append(a.elapsed_time(b) / 5)
+    return min(times)
+
+
+@pytest.mark.parametrize("rows,cols,spread,settings", [(1, 32768, 1.0, dict(temperature=2.0, min_p=0.001)), (64, 131072, 0.2, dict(min_p=0.05)),
+                                                       (64, 131072, 0.2, dict(min_p=0.05, top_p=0.9)), (64, 50021, 1.0, dict(min_p=1e-9, top_k=3000))])
+def test_min_p_that_cuts_nothing_costs_little(rows, cols, spread, settings):
+    """its border lies below every category: no list is made of it, let alone the search digit by digit that an endless list
+    ends in (some ten times as long).  Draws are those without it."""
+    g = torch.Generator().manual_seed(cols)
+    z = (spread * torch.randn(rows, cols, generator=g)).to(DEV)
+    u = torch.rand(rows, generator=g).to(DEV)
+    without = {k: v for k, v in settings.items() if k != "min_p"}
+    cases.check_sample(z[:4], u[:4], **settings)
+    assert torch.equal(ops.sample_logits(z, u, **settings), ops.sample_logits(z, u, **without))
+    slow, base = milliseconds(lambda: ops.sample_logits(z, u, **settings)), milliseconds(lambda: ops.sample_logits(z, u, **without))
+    assert slow < 2 * base, (slow, base)
+
+
+def test_draws_below_the_steps():
+    """logits far apart after a stretch of close ones: borders and draws among those that lie below all steps, few (one list)
+    or many of them"""
+    g = torch.Generator().manual_seed(11)
+    for cols, low in ((9001, 1500), (9001, 4500), (70001, 1900), (70001, 35000)):
+        z = 1e-3 * torch.randn(6, cols, generator=g)
+        z[:, cols - low:] -= 0.3 + 3 * torch.rand(6, low, generator=g)
+        for t in (z, z.bfloat16()):
+            for u in (0.3, 0.7, 0.95, 0.9999):
+                for settings in (dict(), dict(top_p=0.9), dict(min_p=0.3), dict(min_p=0.3, top_p=0.8), dict(top_k=cols - 700), dict(top_k=cols - 700, min_p=0.01)):
+                    cases.check_sample(t.to(DEV), torch.full((6,), u, device=DEV), **settings)
