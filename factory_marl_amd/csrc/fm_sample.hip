@@ -116,15 +116,15 @@ __device__ __forceinline__ uint64_t weight_of(float v, float top, const Row& o) 
   return (uint64_t)__double_as_longlong(fma(exp_neg(x), o.one, 4503599627370496.0)) & 0xfffffffffffffull;
 }
 
-// the number to pass for the share u of `sum`
+// the number to pass for the share u of `sum` (a NaN, whose row is not drawn, gives 0)
 __device__ __forceinline__ uint64_t target_of(double u, uint64_t sum) {
   const double t = u * (double)sum;
-  return t <= 0 ? 0 : t >= (double)sum ? sum - 1 : (uint64_t)t;
+  return !(t > 0) ? 0 : t >= (double)sum ? sum - 1 : (uint64_t)t;
 }
 // the last category kept by top_p passes this number: its own weight starts below p times `sum`
 __device__ __forceinline__ uint64_t border_of(double p, uint64_t sum) {
   const double t = ceil(p * (double)sum);
-  return t <= 1 ? 0 : t >= (double)sum ? sum - 1 : (uint64_t)t - 1;
+  return !(t > 1) ? 0 : t >= (double)sum ? sum - 1 : (uint64_t)t - 1;
 }
 
 // The row's logits, -inf where a category is barred.  The pointers say that they are to global memory, also in functions of
@@ -688,7 +688,8 @@ __device__ __forceinline__ void weigh_steps(const S& src, const Steps& steps, do
     seen |= v != v;
     if (COUNT) categories += v > -INFINITY;
     const double t = fma(-(double)v, steps.scale, base);
-    const uint32_t at = (uint32_t)t;  // (less than 0 and NaN: 0)
+    uint32_t at;  // by the instruction, which gives 0 for less than 0 and NaN, the most for more: in C++ that is undefined
+    asm("v_cvt_u32_f64 %0, %1" : "=v"(at) : "v"(t));
     const uint32_t b = at < BINS - 1 ? at : spare;
     if (COUNT) atomicAdd(&g.count[b], 1u);
     if (WEIGH) {

@@ -106,3 +106,22 @@ def test_draws_below_the_steps():
             for u in (0.3, 0.7, 0.95, 0.9999):
                 for settings in (dict(), dict(top_p=0.9), dict(min_p=0.3), dict(min_p=0.3, top_p=0.8), dict(top_k=cols - 700), dict(top_k=cols - 700, min_p=0.01)):
                     cases.check_sample(t.to(DEV), torch.full((6,), u, device=DEV), **settings)
+
+
+@pytest.mark.parametrize("cols", [2, 50, 700, 5003, 70001])
+def test_settings_and_logits_that_are_no_numbers_leave_other_rows_alone(cols):
+    """NaN and infinities among u, the settings and the logits, above and below the first vectors' largest"""
+    inf, nan = float("inf"), float("nan")
+    g = torch.Generator().manual_seed(cols)
+    z, u = 3 * torch.randn(40, cols, generator=g), torch.rand(40, generator=g)
+    p = torch.full((40,), 0.9)
+    z[1, -1], z[2, 0], z[3, cols // 2], z[4, -1], u[5], p[6] = nan, nan, inf, -inf, nan, nan
+    z[7, 1:] = -inf
+    z[8, -1] = 3e38
+    z[9] = -3e38
+    z[9, cols // 3] = 3e38
+    barred = torch.ones(40, cols, dtype=torch.bool)
+    barred[10, 0] = False
+    z[10, 0] = nan
+    got = cases.check_sample(z.to(DEV), u.to(DEV), mask=barred.to(DEV), top_p=p.to(DEV))
+    assert got[1] == got[2] == got[5] == got[6] == -1 and (got[[3, 4, 7, 8, 9]] >= 0).all()
