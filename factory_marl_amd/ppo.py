@@ -137,9 +137,14 @@ class ActorCriticPolicy(nn.Module):
             for logits in self.action_logits(head):
                 u = torch.rand(logits.shape[:-1], device=head.device, generator=generator)
                 outs.append(ops.sample_logits(logits, u, **settings))
-            # a policy that has become NaN draws -1 throughout: category 0 keeps the actions in range, their
-            # log-probabilities stay NaN
-            return torch.cat(outs, 1).clamp(min=0).to(torch.float32)
+            acts = torch.cat(outs, 1)
+            # a policy that has become NaN draws -1: an error, as torch.multinomial's below (which waits for the GPU too).  A
+            # graph that is being captured cannot wait: there category 0 keeps the actions in range
+            if acts.is_cuda and torch.cuda.is_current_stream_capturing():
+                acts = acts.clamp(min=0)
+            elif (acts < 0).any():
+                raise RuntimeError("nothing to draw: the policy's logits hold NaN, or -inf throughout")
+            return acts.to(torch.float32)
         if self.discrete:
             outs, o = [], 0
             for n in self.nvec:
