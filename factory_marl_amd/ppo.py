@@ -191,17 +191,26 @@ class ActorCriticPolicy(nn.Module):
         head, _ = self._dist_params(obs)
         return self._sample(head, deterministic, generator, **settings)
 
+    def _listed(self, k):
+        """refuses a k that top_logits cannot give"""
+        if k is not None and k < 1:
+            raise ValueError("k is at least 1 (None: every category)")
+        most = max(min(k or n, n) for n in self.nvec)
+        if most > ops.MAX_LISTED:
+            raise ValueError(f"{most} categories to list for an action dimension, at most {ops.MAX_LISTED} can be: give a smaller k")
+
     @torch.no_grad()
     def top_logits(self, obs, k=None):
         """what a student of this MultiDiscrete policy learns from: (category indices, logits) of the k largest logits
         of every action dimension (all of them without k), a pair of [batch, dimensions, k] tensors for each run of
-        equal dimensions (``action_logits``)"""
+        equal dimensions (``action_logits``); at most ``ops.MAX_LISTED`` for each"""
         if not self.discrete:
             raise ValueError("top_logits needs a MultiDiscrete policy")
+        self._listed(k)
         head = self.action_net(self.mlp_extractor.policy_net(obs.float()))
         out = []
         for logits in self.action_logits(head):
-            top = logits.topk(min(k or logits.shape[-1], logits.shape[-1], ops.MAX_LISTED), -1)
+            top = logits.topk(min(k or logits.shape[-1], logits.shape[-1]), -1)
             out.append((top.indices, top.values))
         return out
 
@@ -259,6 +268,8 @@ class PPO:
             raise ValueError("teacher: a MultiDiscrete policy with the student's nvec and observations is needed")
         if distill_top_k is not None and distill_top_k < 1:
             raise ValueError("distill_top_k is at least 1 (None: every category)")
+        if teacher is not None:
+            teacher._listed(distill_top_k)
         self.teacher = None if teacher is None else teacher.to(self.device)
         self.optimizer = torch.optim.Adam(self.policy.parameters(), lr=learning_rate, eps=1e-5)
         self.hp = dict(learning_rate=learning_rate, n_steps=n_steps, batch_size=batch_size, n_epochs=n_epochs,

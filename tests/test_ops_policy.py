@@ -2,6 +2,7 @@
 import pytest
 import torch
 
+from factory_marl_amd import ops
 from factory_marl_amd.ppo import PPO, ActorCriticPolicy
 from test_ppo import ToyEnv
 
@@ -26,3 +27,26 @@ def test_a_policy_that_has_become_nan_raises_where_it_draws():
         ppo.policy.action_net.weight[0, 0] = float("nan")
     with pytest.raises(RuntimeError):
         ppo.collect_rollouts()
+
+
+def test_top_logits_are_as_many_as_asked_for():
+    n = ops.MAX_LISTED + 1
+    pol = ActorCriticPolicy(5, nvec=[n, 4], net_arch=(8,))
+    obs = torch.randn(3, 5)
+    many, few = pol.top_logits(obs, 7)
+    assert many[0].shape == (3, 1, 7) and few[0].shape == (3, 1, 4)
+    assert pol.top_logits(obs, ops.MAX_LISTED)[0][1].shape == (3, 1, ops.MAX_LISTED)
+    for k in (None, n, n + 5, 0, -1):  # more than a list of distill_loss holds, or none
+        with pytest.raises(ValueError):
+            pol.top_logits(obs, k)
+    small = ActorCriticPolicy(5, nvec=[2, 2, 2], net_arch=(8,))
+    assert small.top_logits(obs)[0][0].shape == small.top_logits(obs, 5000)[0][0].shape == (3, 3, 2)
+
+
+@pytest.mark.parametrize("top", [None, ops.MAX_LISTED + 1])
+def test_a_teacher_with_more_categories_than_a_list_holds_needs_top_k(top):
+    nvec = [ops.MAX_LISTED + 1]
+    student, teacher = (ActorCriticPolicy(5, nvec=nvec, net_arch=(8,)) for _ in range(2))
+    with pytest.raises(ValueError):
+        PPO(ToyEnv(n=4, discrete=True), policy=student, teacher=teacher, distill_top_k=top)
+    PPO(ToyEnv(n=4, discrete=True), policy=student, teacher=teacher, distill_top_k=16)
