@@ -321,7 +321,7 @@ void cpu_distill_backward(const fm_distill_args& a) {
     const double mass = teacher_row(a, r, p, logp), scale = a.grad[r * a.grad_stride] * a.temperature;
     for (int64_t c = 0; c < a.cols; c++) {
       const double z = load(a.logits, a.dtype, r * a.stride + c);
-      d[c] = mass == 0 ? 0 : mass * (z == -INFINITY ? 0.0 : std::exp((z - top) / a.temperature) / sum);
+      d[c] = mass == 0 ? 0 : mass * ((z == -INFINITY ? 0.0 : std::exp((z - top) / a.temperature)) / sum);
     }
     for (int64_t i = 0; i < a.k && mass > 0; i++)
       if (p[i] > 0) d[load_index(a.index, a.index_dtype, r * a.index_stride + i)] -= p[i];

@@ -212,7 +212,8 @@ def distill_loss(logits, teacher_index, teacher_logits, temperature=1.0):
     categories and teacher_logits [..., k] (a float dtype of its own) their logits, k at most 1024, in any order.  An
     entry with a negative index or a teacher logit of -inf is not listed (lists of unequal length are padded so); a row
     with none has loss 0 and gradient 0.  A category listed twice counts twice.  An index that is no category cannot be raised
-    without waiting for the GPU: it makes its row's loss and gradient NaN.  Differentiable once in the logits; the
+    without waiting for the GPU: it makes its row's loss and gradient NaN, as do logits without a softmax (all -inf, or
+    NaN or +inf among them or the listed teacher's).  Differentiable once in the logits; the
     teacher's logits are constants."""
     _float_input("logits", logits)
     _float_input("teacher_logits", teacher_logits)

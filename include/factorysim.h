@@ -303,7 +303,8 @@ int64_t fm_sample_workspace(int64_t rows, int64_t cols);
 /* loss[i] = T^2 * sum over the listed entries of p (log p - log q[index]), q = softmax(logits / T) over all columns,
  * p = softmax(teacher / T) over the row's listed entries.  An entry with a negative index or a teacher logit of -inf
  * is not listed; a row without entries has loss 0 and gradient 0; an index >= cols makes the row's loss and
- * gradient NaN; the same index listed twice counts twice.  Backward: dlogits = grad[i] * T * (q - p at the listed places). */
+ * gradient NaN, and so does a row without a softmax (logits all -inf, or +inf or NaN among them; +inf or NaN among the listed
+ * teacher logits); the same index listed twice counts twice.  Backward: dlogits = grad[i] * T * (q - p at the listed places). */
 typedef struct fm_distill_args {
   int32_t device, dtype, index_dtype, teacher_dtype; /* index_dtype: I32 or I64; teacher: F32, F16 or BF16 */
   int64_t rows, cols, k;                             /* 1 <= cols <= FM_MAX_COLS, 1 <= k <= FM_DISTILL_MAX_K */

@@ -4,6 +4,7 @@ import pytest
 
 torch = pytest.importorskip("torch")
 import ops_cases as cases  # noqa: E402
+import test_ops_edges as plain  # noqa: E402
 from factory_marl_amd import ops  # noqa: E402
 
 pytestmark = [pytest.mark.gpu, pytest.mark.skipif(not torch.cuda.is_available(), reason="needs an MI355X")]
@@ -125,3 +126,7 @@ def test_settings_and_logits_that_are_no_numbers_leave_other_rows_alone(cols):
     z[10, 0] = nan
     got = cases.check_sample(z.to(DEV), u.to(DEV), mask=barred.to(DEV), top_p=p.to(DEV))
     assert got[1] == got[2] == got[5] == got[6] == -1 and (got[[3, 4, 7, 8, 9]] >= 0).all()
+
+
+def test_rows_of_the_student_without_a_softmax():
+    plain.check_softmaxless(DEV)
