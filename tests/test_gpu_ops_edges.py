@@ -130,3 +130,14 @@ def test_settings_and_logits_that_are_no_numbers_leave_other_rows_alone(cols):
 
 def test_rows_of_the_student_without_a_softmax():
     plain.check_softmaxless(DEV)
+
+
+@pytest.mark.parametrize("rows,cols", [(300, 5), (300, 128), (50, 1001), (30, 9000), (20, 20000)])
+def test_norm_gradients_wanted_in_part(rows, cols):
+    """each gradient alone, or two of them, has the bits that it has among all three"""
+    x, w, b, dy = cases.norm_inputs(rows, cols, torch.bfloat16, torch.float32, DEV)
+    full = torch.autograd.grad(ops.layer_norm(*(leaves := [v.clone().requires_grad_() for v in (x, w, b)])), leaves, dy)
+    for wanted in ((0,), (1,), (2,), (0, 1), (0, 2), (1, 2)):
+        args = [v.clone().requires_grad_(i in wanted) for i, v in enumerate((x, w, b))]
+        got = torch.autograd.grad(ops.layer_norm(*args), [args[i] for i in wanted], dy)
+        assert all(torch.equal(a, full[i]) for a, i in zip(got, wanted)), wanted
