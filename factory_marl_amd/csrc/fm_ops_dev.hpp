@@ -107,11 +107,10 @@ __device__ __forceinline__ V sum_lanes(V v, int j) {
   return v;
 }
 
-// over a block of NT threads; `buf` holds NT / 64 values and may be used again after the next barrier
+// over a block of NT > 64 threads; `buf` holds NT / 64 values and may be used again after the next barrier
 template <int NT, typename V>
 __device__ __forceinline__ V block_sum(V v, V* buf) {
   v = group_sum<64>(v);
-  if (NT == 64) return v;
   if ((threadIdx.x & 63) == 0) buf[threadIdx.x >> 6] = v;
   __syncthreads();
   return group_sum<NT / 64>(buf[threadIdx.x % (NT / 64)]);
@@ -119,7 +118,6 @@ __device__ __forceinline__ V block_sum(V v, V* buf) {
 template <int NT>
 __device__ __forceinline__ float block_max(float v, float* buf) {
   v = group_max<64>(v);
-  if (NT == 64) return v;
   if ((threadIdx.x & 63) == 0) buf[threadIdx.x >> 6] = v;
   __syncthreads();
   return group_max<NT / 64>(buf[threadIdx.x % (NT / 64)]);

@@ -1245,7 +1245,7 @@ void launch(const fm_sample_args& a) {
 
 using namespace fm;
 extern "C" {
-int64_t fm_sample_workspace(int64_t rows, int64_t cols) { return 0; }
+int64_t fm_sample_workspace(int64_t, int64_t) { return 0; }
 
 int fm_sample_logits(const fm_sample_args* a) {
   return guarded([&] {

@@ -39,7 +39,6 @@ struct Entries {
   decltype(&fm_distill_backward) distill_backward;
   decltype(&fm_distill_workspace) distill_workspace;
   decltype(&fm_sample_logits) sample_logits;
-  decltype(&fm_sample_workspace) sample_workspace;
   decltype(&fm_last_error) last_error;
 } fm;
 
@@ -342,7 +341,6 @@ Tensor sample_logits(const Tensor& z_, const Tensor& u_, const Maybe& mask_, dou
   a.min_p_rows = (const float*)data(m_rows);
   Tensor out = at::empty({a.rows}, z.options().dtype(at::kLong));
   a.out = (int64_t*)data(out);
-  const Tensor work = workspace(a, fm.sample_workspace(a.rows, a.cols), z);
   check(fm.sample_logits(&a));
   return out;
 }

@@ -40,7 +40,7 @@ def _library():
             raise _lib.FactorySimError(f"{_NODES} not built: run `python __graft_entry__.py build`")
         torch.ops.load_library(_NODES)
         names = ("fm_layer_norm_forward", "fm_layer_norm_backward", "fm_layer_norm_workspace", "fm_distill_forward",
-                 "fm_distill_backward", "fm_distill_workspace", "fm_sample_logits", "fm_sample_workspace", "fm_last_error")
+                 "fm_distill_backward", "fm_distill_workspace", "fm_sample_logits", "fm_last_error")
         addresses = (C.c_void_p * len(names))(*(C.cast(getattr(L, n), C.c_void_p).value for n in names))
         bind = C.CDLL(_NODES).fm_torch_bind
         bind.argtypes, bind.restype = [C.POINTER(C.c_void_p), C.c_int64], C.c_bool
