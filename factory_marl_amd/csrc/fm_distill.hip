@@ -191,8 +191,7 @@ __global__ __launch_bounds__(NT) void distill_fwd_group(const T* z, int64_t stri
 // the one entry, or, where a column is listed twice (a bit of it is set twice), by all entries' sum, the same for each of them.
 template <typename T, int G, bool WIDE>
 __global__ __launch_bounds__(NT) void distill_bwd_group(const T* z, int64_t stride, Teacher t, const float* stats,
-    const float* grad, int64_t grad_stride,
-                                                        T* dz, int64_t rows) {
+    const float* grad, int64_t grad_stride, T* dz, int64_t rows) {
   constexpr int N = 16 / (int)sizeof(T), WORDS = WIDE ? SHORT / 32 : G / 32 + (G < 32);
   __shared__ uint32_t bits[NT / G][WORDS];
   const int lane = threadIdx.x & 63, j = lane & (G - 1), base = lane - j;
@@ -268,8 +267,7 @@ __device__ __forceinline__ Softmax block_softmax(const T* zr, int from, int to, 
 
 template <typename T>
 __device__ __forceinline__ void write_loss(const T* zr, const Teacher& t, int64_t r, const Softmax& q, float* loss,
-    float* stats, int* at, float* p, float* buf,
-                                           double* dbuf) {
+    float* stats, int* at, float* p, float* buf, double* dbuf) {
   float top, total;
   const float mass = load_teacher(t, r, at, p, buf, top, total);
   const double log_ratio = log((double)q.s / total);
@@ -332,9 +330,8 @@ __global__ __launch_bounds__(NT) void distill_fwd_join(const T* z, int64_t strid
 // dlogits of a split of a row a block: everything first as if nothing were listed, then the listed columns of the split
 // again, as above (whoever lists the same one writes the same value).
 template <typename T>
-__global__ __launch_bounds__(NT) void distill_bwd(const T* z, int64_t stride, Teacher t, const float* stats, const float* grad,
-    int64_t grad_stride, T* dz,
-                                                  int64_t rows, int splits) {
+__global__ __launch_bounds__(NT) void distill_bwd(const T* z, int64_t stride, Teacher t, const float* stats,
+    const float* grad, int64_t grad_stride, T* dz, int64_t rows, int splits) {
   __shared__ int at[FM_DISTILL_MAX_K];
   __shared__ float p[FM_DISTILL_MAX_K], buf[3 * (NT / 64)];
   __shared__ uint32_t seen[SPLIT / 32 + 1], dup[SPLIT / 32 + 1];  // columns of the split that are listed, and listed twice
@@ -435,8 +432,8 @@ void forward(const fm_distill_args& a) {
   const T* z = (const T*)a.logits;
   if (with_group(a.cols, a.k, [&](auto g, auto w) {
         const int64_t n = (a.rows + NT / g - 1) / (NT / g);
-        distill_fwd_group<T, decltype(g)::value, decltype(w)::value><<<(int)(n < (1 << 20) ? n : 1 << 20), NT, 0,
-            st>>>(z, a.stride, t, a.loss, a.stats, a.rows);
+        distill_fwd_group<T, decltype(g)::value, decltype(w)::value><<<(int)(n < (1 << 20) ? n : 1 << 20), NT, 0, st>>>(z,
+            a.stride, t, a.loss, a.stats, a.rows);
       }))
     return;
   const int splits = splits_of(a.rows, a.cols);
@@ -455,16 +452,15 @@ void backward(const fm_distill_args& a) {
   const T* z = (const T*)a.logits;
   if (with_group(a.cols, a.k, [&](auto g, auto w) {
         const int64_t n = (a.rows + NT / g - 1) / (NT / g);
-        distill_bwd_group<T, decltype(g)::value, decltype(w)::value>
-            <<<(int)(n < (1 << 20) ? n : 1 << 20), NT, 0,
-                st>>>(z, a.stride, t, a.stats, a.grad, a.grad_stride, (T*)a.dlogits, a.rows);
+        distill_bwd_group<T, decltype(g)::value, decltype(w)::value><<<(int)(n < (1 << 20) ? n : 1 << 20), NT, 0, st>>>(z,
+            a.stride, t, a.stats, a.grad, a.grad_stride, (T*)a.dlogits, a.rows);
       }))
     return;
   // a block for every SPLIT columns (the list is read again for each), for fewer where that leaves CUs without work
   int64_t splits = (a.cols + SPLIT - 1) / SPLIT;
   if (a.rows * splits < 1024) splits = splits_of(a.rows, a.cols) > splits ? splits_of(a.rows, a.cols) : splits;
-  distill_bwd<T><<<grid_of(a.rows * splits), NT, 0,
-      st>>>(z, a.stride, t, a.stats, a.grad, a.grad_stride, (T*)a.dlogits, a.rows, (int)splits);
+  distill_bwd<T><<<grid_of(a.rows * splits), NT, 0, st>>>(z, a.stride, t, a.stats, a.grad, a.grad_stride, (T*)a.dlogits,
+      a.rows, (int)splits);
 }
 }  // namespace
 }  // namespace fm

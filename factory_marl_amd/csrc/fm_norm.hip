@@ -61,8 +61,7 @@ __device__ __forceinline__ void each_vector(int cols, F&& f) {
 
 template <typename T, typename P>
 __global__ __launch_bounds__(WT) void norm_fwd_wide(const T* x, int64_t x_stride, const P* weight, const P* bias, T* y,
-    float* mean_out,
-                                                    float* rstd_out, int64_t rows, int cols, float eps) {
+    float* mean_out, float* rstd_out, int64_t rows, int cols, float eps) {
   constexpr int N = 16 / (int)sizeof(T);
   __shared__ float buf[2][WT / 64];
   for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
@@ -103,8 +102,7 @@ __global__ __launch_bounds__(WT) void norm_fwd_wide(const T* x, int64_t x_stride
 
 template <typename T, typename P>
 __global__ __launch_bounds__(WT) void norm_dx_wide(const T* x, int64_t x_stride, const T* dy, int64_t dy_stride,
-    const P* weight, const float* mean_in,
-                                                   const float* rstd_in, T* dx, int64_t rows, int cols) {
+    const P* weight, const float* mean_in, const float* rstd_in, T* dx, int64_t rows, int cols) {
   constexpr int N = 16 / (int)sizeof(T);
   __shared__ float buf[2][WT / 64];
   for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
@@ -140,8 +138,7 @@ __global__ __launch_bounds__(WT) void norm_dx_wide(const T* x, int64_t x_stride,
 // Sums over a stretch of rows, 64 columns a block, 4 rows at a time: part[stretch] = dweight, dbias of the stretch.
 template <typename T>
 __global__ __launch_bounds__(NT) void norm_dparam_wide(const T* x, int64_t x_stride, const T* dy, int64_t dy_stride,
-    const float* mean_in,
-                                                       const float* rstd_in, float* part, int64_t rows, int cols) {
+    const float* mean_in, const float* rstd_in, float* part, int64_t rows, int cols) {
   __shared__ float buf[2][4][64];
   const int c = blockIdx.x * 64 + (threadIdx.x & 63), lane = threadIdx.x >> 6;
   const int64_t each = (rows + gridDim.y - 1) / gridDim.y, first = blockIdx.y * each;
@@ -218,8 +215,7 @@ __device__ __forceinline__ float row_sum(float v, float* buf) {
 
 template <typename T, typename P, int NT_, int TPR, int V, int N>
 __global__ __launch_bounds__(NT_) void norm_fwd(const T* x, int64_t x_stride, const P* weight, const P* bias, T* y,
-    float* mean_out, float* rstd_out,
-                                                int64_t rows, int cols, float eps) {
+    float* mean_out, float* rstd_out, int64_t rows, int cols, float eps) {
   constexpr int RPB = NT_ / TPR;
   __shared__ float buf[2][2][NT_ / 64];
   const int t = threadIdx.x % TPR;
@@ -278,9 +274,8 @@ __global__ __launch_bounds__(NT_) void norm_fwd(const T* x, int64_t x_stride, co
 // (16384 x 8192 bf16: 266 us), whole ones and the next row ahead take 152.
 // The columns' sums of a block's rows are joined over its wave's lanes, then over its waves through LDS, in order.
 template <typename T, typename P, int NT_, int TPR, int V, int N>
-__global__ __launch_bounds__(NT_) void norm_bwd(const T* x, int64_t x_stride, const T* dy, int64_t dy_stride, const P* weight,
-    const float* mean_in,
-                                                const float* rstd_in, T* dx, float* part, int64_t rows, int cols) {
+__global__ __launch_bounds__(NT_) void norm_bwd(const T* x, int64_t x_stride, const T* dy, int64_t dy_stride,
+    const P* weight, const float* mean_in, const float* rstd_in, T* dx, float* part, int64_t rows, int cols) {
   constexpr int RPB = NT_ / TPR;
   __shared__ float buf[2][2][NT_ / 64];
   extern __shared__ float sums[];  // [groups of rows][cols], for one of the two at a time
@@ -467,17 +462,15 @@ void forward(const fm_layer_norm_args& a) {
   hipStream_t st = (hipStream_t)a.stream;
   const int cols = (int)a.cols;
   if (cols > WIDEST) {
-    norm_fwd_wide<T, P><<<(int)(a.rows < (1 << 20) ? a.rows : 1 << 20), WT, 0,
-        st>>>((const T*)a.x, a.x_stride, (const P*)a.weight, (const P*)a.bias, (T*)a.y,
-              a.mean, a.rstd, a.rows, cols, (float)a.eps);
+    norm_fwd_wide<T, P><<<(int)(a.rows < (1 << 20) ? a.rows : 1 << 20), WT, 0, st>>>((const T*)a.x, a.x_stride,
+        (const P*)a.weight, (const P*)a.bias, (T*)a.y, a.mean, a.rstd, a.rows, cols, (float)a.eps);
     return;
   }
   with_shape<T>(a.cols, [&](auto nt, auto tpr, auto n, auto e) {
     constexpr int B = decltype(nt)::value, TPR = decltype(tpr)::value, V = decltype(n)::value, N = decltype(e)::value;
     const int64_t turns = (a.rows + B / TPR - 1) / (B / TPR), most = 256 * 2048 / B;
-    norm_fwd<T, P, B, TPR, V, N><<<(int)(turns < most ? turns : most), B, 0,
-        st>>>((const T*)a.x, a.x_stride, (const P*)a.weight, (const P*)a.bias, (T*)a.y, a.mean,
-                                                                                a.rstd, a.rows, cols, (float)a.eps);
+    norm_fwd<T, P, B, TPR, V, N><<<(int)(turns < most ? turns : most), B, 0, st>>>((const T*)a.x, a.x_stride,
+        (const P*)a.weight, (const P*)a.bias, (T*)a.y, a.mean, a.rstd, a.rows, cols, (float)a.eps);
   });
 }
 
@@ -489,27 +482,25 @@ void backward(const fm_layer_norm_args& a) {
   int parts = 0;
   if (a.rows > 0 && cols > WIDEST) {
     if (a.dx)
-      norm_dx_wide<T, P><<<(int)(a.rows < (1 << 20) ? a.rows : 1 << 20), WT, 0,
-          st>>>((const T*)a.x, a.x_stride, (const T*)a.dy, a.dy_stride, (const P*)a.weight,
-                                                                                      a.mean, a.rstd, (T*)a.dx, a.rows, cols);
+      norm_dx_wide<T, P><<<(int)(a.rows < (1 << 20) ? a.rows : 1 << 20), WT, 0, st>>>((const T*)a.x, a.x_stride,
+          (const T*)a.dy, a.dy_stride, (const P*)a.weight, a.mean, a.rstd, (T*)a.dx, a.rows, cols);
     parts = wide_parts(a.rows);
     if (sums)
-      norm_dparam_wide<T><<<dim3((cols + 63) / 64, parts), NT, 0,
-          st>>>((const T*)a.x, a.x_stride, (const T*)a.dy, a.dy_stride, a.mean, a.rstd,
-                                                                        (float*)a.workspace, a.rows, cols);
+      norm_dparam_wide<T><<<dim3((cols + 63) / 64, parts), NT, 0, st>>>((const T*)a.x, a.x_stride, (const T*)a.dy,
+          a.dy_stride, a.mean, a.rstd, (float*)a.workspace, a.rows, cols);
   } else if (a.rows > 0 && (a.dx || sums)) {
     with_shape<T>(a.cols, [&](auto nt, auto tpr, auto n, auto e) {
       constexpr int B = decltype(nt)::value, TPR = decltype(tpr)::value, V = decltype(n)::value, N = decltype(e)::value;
       parts = blocks_of(a.rows, B / TPR, B);
-      norm_bwd<T, P, B, TPR, V, N><<<parts, B, B > TPR ? 4 * cols * (TPR < 64 ? B / 64 : B / TPR) : 0,
-          st>>>((const T*)a.x, a.x_stride, (const T*)a.dy, a.dy_stride, (const P*)a.weight, a.mean,
-                a.rstd, (T*)a.dx, sums ? (float*)a.workspace : nullptr, a.rows, cols);
+      norm_bwd<T, P, B, TPR, V, N><<<parts, B, B > TPR ? 4 * cols * (TPR < 64 ? B / 64 : B / TPR) : 0, st>>>((const T*)a.x,
+          a.x_stride, (const T*)a.dy, a.dy_stride, (const P*)a.weight, a.mean, a.rstd, (T*)a.dx,
+          sums ? (float*)a.workspace : nullptr, a.rows, cols);
     });
   }
   if (!sums) return;
   if (cols > 1)
-    norm_dparam_sum<P, 4><<<grid_of((2 * (int64_t)cols + 63) / 64), ST, 0,
-        st>>>((const float*)a.workspace, parts, (P*)a.dweight, (P*)a.dbias, cols);
+    norm_dparam_sum<P, 4><<<grid_of((2 * (int64_t)cols + 63) / 64), ST, 0, st>>>((const float*)a.workspace, parts,
+        (P*)a.dweight, (P*)a.dbias, cols);
   else
     norm_dparam_sum<P, 1><<<1, ST, 0, st>>>((const float*)a.workspace, parts, (P*)a.dweight, (P*)a.dbias, cols);
 }

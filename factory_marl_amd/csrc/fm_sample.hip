@@ -204,9 +204,8 @@ __device__ __forceinline__ uint64_t sort_lanes(uint64_t p, int j) {
 // G lanes a row, one category each: sorted by exchanging places between lanes, then every setting is a prefix of the
 // group's lanes.  Rows of two categories fill a wave 32 at a time: 65536 of them take 5 us, of 33 categories 42.
 template <typename T, int G>
-__global__ __launch_bounds__(256) void sample_group(const T* logits, int64_t stride, const uint8_t* mask, int64_t mask_stride,
-    Settings a, int64_t* out,
-                                                    int64_t rows, int cols) {
+__global__ __launch_bounds__(256) void sample_group(const T* logits, int64_t stride, const uint8_t* mask,
+    int64_t mask_stride, Settings a, int64_t* out, int64_t rows, int cols) {
   const int lane = threadIdx.x & 63, j = lane & (G - 1), base = lane - j;
   const uint64_t group = (G == 64 ? ~0ull : (1ull << G) - 1) << base;
   const int64_t step = (int64_t)gridDim.x * (256 / G);
@@ -480,8 +479,7 @@ struct WaveRow {
 
 template <typename T, bool MASKED, int R>
 __global__ __launch_bounds__(256, R > 16 ? 2 : 4) void sample_wave(const T* logits, int64_t stride, const uint8_t* mask,
-    int64_t mask_stride, Settings a, int64_t* out,
-                                                                 int64_t rows, int cols) {
+    int64_t mask_stride, Settings a, int64_t* out, int64_t rows, int cols) {
   typedef WaveRow<T, MASKED, R> W;
   constexpr int N = W::N;
   __shared__ typename W::Lds lds[4];
@@ -1025,9 +1023,8 @@ __device__ __forceinline__ uint64_t draw_by_steps(const Steps& steps, float top,
 }
 
 template <typename T, bool MASKED, int NT>
-__global__ __launch_bounds__(NT, 4) void sample_long(const T* logits, int64_t stride, const uint8_t* mask, int64_t mask_stride,
-    Settings a, int64_t* out,
-                                                  int64_t rows, int cols) {
+__global__ __launch_bounds__(NT, 4) void sample_long(const T* logits, int64_t stride, const uint8_t* mask,
+    int64_t mask_stride, Settings a, int64_t* out, int64_t rows, int cols) {
   Long<NT>& g = shared<NT>();
   const int64_t r = blockIdx.x + (int64_t)gridDim.x * blockIdx.y;
   if (r >= rows) return;
