@@ -466,8 +466,14 @@ struct DistillBackward : public torch::autograd::Node {
   std::string name() const override { return "DistillBackward"; }
 };
 
+// the teacher's logits are constants: their gradient would be lost without a word
+void constant(const Tensor& teacher) {
+  TORCH_CHECK(!torch::autograd::compute_requires_grad(teacher),
+              "factorysim: teacher_logits requires a gradient, which this loss does not give: detach it");
+}
+
 Two distill_loss_stats(const Tensor& z, const Tensor& index, const Tensor& teacher, double temperature) {
-  no_tangent(z), no_tangent(teacher);
+  no_tangent(z), no_tangent(teacher), constant(teacher);
   const bool wanted = torch::autograd::compute_requires_grad(z);
   Two out;
   {
@@ -488,7 +494,7 @@ Two distill_loss_stats(const Tensor& z, const Tensor& index, const Tensor& teach
 
 Tensor distill_loss(const Tensor& z, const Tensor& index, const Tensor& teacher, double temperature) {
   if (torch::autograd::compute_requires_grad(z)) return std::get<0>(distill_loss_stats(z, index, teacher, temperature));
-  no_tangent(z), no_tangent(teacher);
+  no_tangent(z), no_tangent(teacher), constant(teacher);
   at::AutoDispatchBelowADInplaceOrView below;
   return CALL(distill_loss, z, index, teacher, temperature);
 }

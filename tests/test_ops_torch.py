@@ -204,6 +204,17 @@ def test_direct_calls_are_checked():
     assert torch.equal(broad, ops.sample_logits(z, u, mask=(z > 0)[0]))
 
 
+def test_a_teacher_that_wants_a_gradient_is_refused_directly_too():
+    ops._library()
+    _, _, _, _, z, at, t, _ = inputs()
+    for op in (torch.ops.factorysim.distill_loss, torch.ops.factorysim.distill_loss_stats):
+        for leaf in (z.clone().requires_grad_(), z):
+            with pytest.raises(RuntimeError, match="detach"):
+                op(leaf, at, t.clone().requires_grad_(), 1.0)
+        with torch.no_grad():
+            op(z, at, t.clone().requires_grad_(), 1.0)
+
+
 def test_the_entry_points_are_no_operator():
     ops._library()
     with pytest.raises(AttributeError):
