@@ -5,8 +5,9 @@
 //
 // The forward pass reads z once (a running maximum and sum), the backward pass reads it again and writes dz: memory bounds both
 // on long rows, the launches (3 us each) on short ones.  Measured on an MI355X: 4096 x 131072 bf16, k 64, 229 us forward
-// (4.7 TB/s; the exponentials come close to the loads there, fp32 reaches 5.9) and 395 us backward (5.4 TB/s, as a copy);
-// 1021 x 50021 bf16, k 37, 27 and 41 us; 32768 x 2, k 2, 3.5 and 3.6 us; 65536 x 64, k 64, 38 and 28 us.
+// (4.7 TB/s; the exponentials come close to the loads there, fp32 reaches 5.9) and 396 us backward (5.4 TB/s, as a copy);
+// 1021 x 50021 bf16, k 37, 27 and 41 us (22 and 36 with z still in the cache); 32768 x 2, k 2, 3.4 and 3.6 us; 65536 x 64, k 64,
+// 39 and 27 us: one row in flight a wave, and a float64 logarithm in each listed lane.
 #include <cfloat>
 #include <type_traits>
 
@@ -393,7 +394,11 @@ Teacher teacher_of(const fm_distill_args& a) {
                  a.temperature * a.temperature};
 }
 
-// splits of a row in the forward pass: where there are fewer rows than fill the chip (4 blocks a CU), of 4096 columns or more
+// splits of a row in the forward pass: where there are fewer rows than fill the chip (4 blocks a CU), of 4096 columns or more.
+// Measured, us without / with them, bf16: 1 x 131072 12.8 / 7.0, 64 x 131072 13.4 / 9.3, 256 x 131072 18.6 / 18.3; but 1 x 8192
+// 5.0 / 6.9, 1 x 32768 6.6 / 6.8, 512 x 32768 10.4 / 13.0, 512 x 131072 25.3 / 30.0: the second launch costs 2 us, so they could
+// begin at some 32768 columns and end at 256 rows.  (backward, which needs no second launch: 1 x 32768 8.2 / 5.5, 256 x 32768
+// 11.8 / 10.8, 512 x 32768 16.7 / 15.4)
 int splits_of(int64_t rows, int64_t cols) {
   if (rows < 1 || rows >= 1024) return 1;
   const int64_t wanted = 1024 / rows, most = cols / 4096;

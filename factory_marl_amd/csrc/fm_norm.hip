@@ -5,8 +5,9 @@
 //
 // Some 20 operations an element against 4 to 16 bytes: memory bounds all of it but the smallest calls, which a launch does
 // (3 us).  Forward reads x and writes y, backward reads x and dy and writes dx: five passes.  Measured on an MI355X, where a
-// copy of 1 GiB moves 5.1 TB/s: 16384 x 8192 bf16 93 us forward (5.8 TB/s) and 152 + 5 us backward (5.3 TB/s);
-// 32768 x 512 fp32 22 and 35 us; 5003 x 1001 fp16, no row aligned, 7.3 and 15 us; 8192 x 128 fp32 4 and 8 us.
+// copy of 1 GiB moves 5.1 TB/s: 16384 x 8192 bf16 91 us forward (5.9 TB/s) and 155 + 5 us backward (5.2 TB/s);
+// 32768 x 512 fp32 21 and 36 us; 5003 x 1001 fp16, no row aligned, 6.9 and 15.5 us (5003 x 1024, all aligned, 6.3 and 14.9: it is
+// the size, a few rows a block, and not the alignment that keeps it from its 4 and 6); 8192 x 128 fp32 4 and 8 us.
 #include <type_traits>
 
 #include "fm_ops_dev.hpp"
@@ -48,7 +49,8 @@ __device__ __forceinline__ void load_param(const P* p, int at, float other, floa
 
 // ---------------------------------------------------------------------------------------------- rows beyond 16384
 // One block a row, the row read again (from the cache) for each of its sums.  Vectors as below: whole, the last one moved back
-// to the row's end; `skip` of its elements are another thread's too.  1024 x 20000 bf16: 31 us forward (2.6 TB/s).
+// to the row's end; `skip` of its elements are another thread's too.  1024 x 20000 bf16: 27 us forward (3.1 TB/s), 28 + 24 + 4
+// backward: x is read three times forward, x and dy three times backward.
 constexpr int WT = 1024;
 template <typename T, typename F>
 __device__ __forceinline__ void each_vector(int cols, F&& f) {
@@ -448,7 +450,8 @@ void with_shape(int64_t cols, F&& f) {
 
 // Blocks of the backward pass, each with sums of its own: one for each of the 256 CUs; of 256 threads twice as many
 // (their registers let two or three share a CU) where a block still gets 8 rows, so that writing and adding up its sums
-// stays small beside them.
+// stays small beside them.  Measured with 256 / 512 blocks, bf16, us: 1024 x 2048 11.3 / 12.8, 8192 x 2048 32.9 / 26.1, 2048 x
+// 1001 10.7 / 12.7, 32768 x 1001 38.9 / 38.0 (256 threads); 1024 x 16384 35.4 / 50.2, 8192 x 16384 163 / 176 (more threads).
 int blocks_of(int64_t rows, int rpb, int threads) {
   const int64_t turns = (rows + rpb - 1) / rpb, most = threads == 256 ? 512 : 256;
   const int64_t blocks = rows / 8 < 256 ? 256 : rows / 8 < most ? rows / 8 : most;

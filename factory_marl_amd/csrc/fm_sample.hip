@@ -6,13 +6,16 @@
 // and so does the share u of the kept weight, so all of them are the same question: which category is the one where a running
 // sum (of ones, or of weights) passes a number.
 //
-// Weights are exp((logit - largest) / T) in multiples of 2^-s of the largest's, as 64-bit integers: sums are exact, so no
-// result depends on the order in which a launch happens to add, and a border that lies 2^-45 of the row's weight away is still
-// told apart (fp32 sums over 10^5 categories lose 2^-20 and would draw another category).
+// Weights are exp((logit - largest) / T) in multiples of 2^-s of the largest's (s = 51 up to 2048 categories, 45 for 2^17), as
+// 64-bit integers whose sums do not depend on the order in which a launch happens to add: a call gives the same on every run.
+// A weight is good to 6e-15 of itself (exp_neg), beyond 2048 categories the sums that find a border's step to 5e-13 (2^-41; fp32
+// sums over 10^5 categories lose 2^-20 and would draw another category).  Where a border lies as near as that to one between two
+// categories, another kernel or backend may draw the neighbour.  Shares of equal logits that hold all the weight are exact.
 //
-// Measured on an MI355X: 16384 x 2 fp32 3.4 us, 16384 x 1000 72, 1 x 32768 15, 37 x 50021 with a mask 25, 256 x 131072 bf16,
-// top_p 0.9, 56, of which reading it once would take 13.  Short rows are bound by their launch, rows of hundreds by the
-// instructions of sorting out one row each, long ones by float64 instructions (17 a logit) and a second read.
+// Measured on an MI355X: 16384 x 2 fp32 3.3 us, 65536 x 33 42, 16384 x 1000 74, 1 x 32768 15, 37 x 50021 with a mask 25,
+// 256 x 131072 bf16, top_p 0.9, 57, of which reading it once would take 13.  Short rows are bound by their launch, 33 to 64
+// categories by the 21 exchanges that sort them, rows of hundreds by a float64 exponential and an LDS atomic a logit, long ones by
+// float64 instructions (17 a logit) and a second read.
 #include <type_traits>
 
 #include "fm_ops_dev.hpp"
@@ -1097,7 +1100,7 @@ __global__ __launch_bounds__(NT, 4) void sample_long(const T* logits, int64_t st
     const double wanted = fmin(fmin(fmax(fmax(32.0 * 1.4426950408889634 * inv_t, close), 1e-30), 64.0 * most), 1e300);
     Steps steps;
     steps.first = uniform(first);
-    steps.scale = uniform(__longlong_as_double(__double_as_longlong(wanted) >> 37 << 37));
+    steps.scale = uniform(__longlong_as_double(__double_as_longlong(wanted) >> 37 << 37));  // 16 bits: first * scale is exact
     steps.inv = uniform(1.0 / steps.scale);
     steps.width = uniform(inv_t * steps.inv);
     steps.base = uniform(steps.first * steps.scale + HEAD);
@@ -1198,8 +1201,12 @@ int shift_of(int64_t cols) {  // the sum of cols weights of at most 2^s stays be
   return s;
 }
 
-// Up to 64 categories a group of lanes holds a row, up to 2048 a wave, longer rows take a block: of 256 threads (four to a
-// CU) where that fills the chip or the row has little for more, else of 1024.
+// Up to 64 categories a group of lanes holds a row, up to 2048 a wave, longer rows take a block: of 256 threads (three to a
+// CU by their LDS) where there are rows enough or the row has little for more, else of 1024 (one to a CU).  Measured with
+// top_p 0.9, us with 256 / 1024 threads: rows of 2100 fp32 16 / 14 for 16 of them, 19 / 27 for 512, 32 / 51 for 1024; of 9001
+// 22 / 18 for 256, 25 / 33 for 512, 47 / 62 for 1024; of 65536 86 / 48 for 256, 83 / 87 for 512, 145 / 159 for 1024; of 131072
+// 131 / 71, 148 / 133 and 300 / 261.  So the one border could lie at 512 rows, and rows up to 4096 would gain 2 us by 1024
+// threads where they are few.
 template <typename T, bool MASKED>
 void launch(const fm_sample_args& a) {
   const Settings s{a.temperature, a.top_p, a.min_p, a.top_k, a.temperature_rows, a.top_p_rows, a.min_p_rows, a.top_k_rows, a.u,

@@ -4,9 +4,10 @@ fm_distill.hip): layer norm, drawing categories from logits, distillation from a
 GPU tensors are computed on torch's current stream of their device, CPU tensors by the library's CPU backend (as
 ``FactoryVecEnv(device=-1)``); there is no other path, a missing library raises.  Inputs may have any leading shape and
 row stride; one whose last dimension is not adjacent in memory is copied first.  Nothing synchronises and no buffer is
-kept between calls, so each call, forward or backward, can be captured into a graph.  A backward pass that is captured needs leaves
-that no live eager graph holds: torch ties a leaf's gradient to the stream of the graph that first used it.  A row has at
-most 2^28 elements.
+kept between calls, so each call, forward or backward, can be captured into a graph.  Calls can be traced and compiled
+(make_fx, torch.compile: each is one operator there) and differentiated by function transforms.  A backward pass that is
+captured needs leaves that no live eager graph holds: torch ties a leaf's gradient to the stream of the graph that first
+used it.  A row has at most 2^28 elements.
 """
 import ctypes as C
 import math
@@ -165,8 +166,10 @@ def sample_logits(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, mas
     gives the largest logit; top_k <= 0, top_p >= 1 and min_p <= 0 are off.  ``mask`` (bool, logits' shape or
     [categories]) bars categories where it is False, whatever their logit; a logit of -inf bars its category too.
     -1 stands for a row with no category left, with NaN in a logit that is not barred, or with a NaN in u or a setting.
-    logits: float32, float16 or bfloat16; u: float32 or float64, in [0, 1).  Weights below 2^-46 of the largest count as
-    nothing (2^-45 beyond 2^17 categories, and a bit less for each doubling)."""
+    logits: float32, float16 or bfloat16; u: float32 or float64, in [0, 1).  Weights below 2^-52 of the largest count as
+    nothing, on the GPU beyond 2048 categories those below e^-33 (2^-47.6), beyond 2^15 below 2^-47, twice that for each doubling.
+    The same call draws the same on every run; where a border falls within 5e-13 of the row's weight of one between two
+    categories, the GPU and the CPU may draw neighbours."""
     _float_input("logits", logits)
     if not torch.is_tensor(u) or u.dtype not in (torch.float32, torch.float64):
         raise TypeError("u is a float32 or float64 tensor")

@@ -276,8 +276,11 @@ int64_t fm_layer_norm_workspace(int64_t rows, int64_t cols);
  * (top_k: int32) of each row's own.
  * temperature <= 0: the largest logit; top_k <= 0, top_p >= 1, min_p <= 0: off; top_p <= 0 and min_p >= 1 keep the
  * largest (min_p: and its equals); u is meant to be in [0, 1) and is cut to what is kept.  Weights are whole multiples of
- * 2^-s of the largest's, s = 51 or what 62 bits leave for the sum of cols of them (45 for 2^17 categories); what weighs
- * less than half of that is never drawn.  Their sums are exact and do not depend on the order. */
+ * 2^-s of the largest's, s = 51 or what 62 bits leave for the sum of cols of them (45 for 2^17 categories), and are added up as
+ * whole numbers, so a call gives the same on every run.  What weighs less than 2^-(s+1) is never drawn, on the GPU beyond
+ * 2048 columns nor what weighs less than e^-33.  Weights are good to 6e-15 of themselves, the GPU's sums beyond 2048
+ * columns to 5e-13: the GPU and the CPU can draw neighbours where a border lies as near as that to one between two
+ * categories (shares of equal logits that hold all the weight are exact). */
 typedef struct fm_sample_args {
   int32_t device, dtype, u_dtype, reserved; /* u_dtype: F32 or F64 */
   int64_t rows, cols;                       /* 1 <= cols <= FM_MAX_COLS */
@@ -298,7 +301,7 @@ typedef struct fm_sample_args {
   void* stream;
 } fm_sample_args;
 int fm_sample_logits(const fm_sample_args* a);
-int64_t fm_sample_workspace(int64_t rows, int64_t cols);
+int64_t fm_sample_workspace(int64_t rows, int64_t cols); /* 0: a draw takes none, workspace is not read */
 
 /* loss[i] = T^2 * sum over the listed entries of p (log p - log q[index]), q = softmax(logits / T) over all columns,
  * p = softmax(teacher / T) over the row's listed entries.  An entry with a negative index or a teacher logit of -inf
