@@ -219,3 +219,24 @@ def test_the_entry_points_are_no_operator():
     ops._library()
     with pytest.raises(AttributeError):
         torch.ops.factorysim.bind
+
+
+# ------------------------------------------------------------------ graphs used more than once
+def test_graphs_kept_changed_and_differentiated_again():
+    x, w, b, dy, z, at, t, g = inputs()
+    for leaf, call, seed in ((x, lambda v: ops.layer_norm(v, w, b), dy), (z, lambda v: ops.distill_loss(v, at, t), g)):
+        a = leaf.clone().requires_grad_()
+        y = call(a)
+        first, = torch.autograd.grad(y, a, seed, retain_graph=True)
+        second, = torch.autograd.grad(y, a, seed)
+        assert torch.equal(first, second)
+        with pytest.raises(RuntimeError, match="second time"):
+            torch.autograd.grad(y, a, seed)
+        y = call(a)
+        with torch.no_grad():
+            a.add_(1)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            torch.autograd.grad(y, a, seed)
+        again, = torch.autograd.grad(call(a), a, seed, create_graph=True)
+        with pytest.raises(RuntimeError, match="differentiable once"):
+            again.sum().backward()
